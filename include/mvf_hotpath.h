@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MVF_ABI_VERSION 14
+#define MVF_ABI_VERSION 15
 
 #if defined(__GNUC__)
 #define MVF_API __attribute__((visibility("default")))
@@ -575,6 +575,55 @@ MVF_API int mvf_color_jitter(const float *img, const float *factors, const int32
                      const int32_t *flip, float *out_raw, float *out_aug, float *workspace, int samples,
                      int frames, int H, int W, void *stream);
 
+/* ---- token attention: norms and position rotation of queries and keys, cross attention ---------------
+ * The attention the fusion of a frame with its neighbours can use (networks/fusion_module.py fuses them by
+ * warping alone: fusion_module.py:100-130); no counterpart in the reference.  Tensors are [batch, token, head,
+ * channel], channels adjacent; strides in ELEMENTS for batch, token and head; at most MVF_ATTN_MAX_D channels
+ * per head; dtype MVF_DTYPE_F32 or MVF_DTYPE_BF16 for everything that is `void *`. */
+#define MVF_DTYPE_F32 0
+#define MVF_DTYPE_BF16 1
+#define MVF_ATTN_MAX_D 128
+
+typedef struct mvf_attn_desc {
+    const void *q, *k, *v;          /* q [B,Lq,Hq,D], k and v [B,Lk,Hk,D]; Hq a multiple of Hk: head h reads h / (Hq/Hk) */
+    const uint8_t *key_mask;        /* nullable [B,Lk] bytes, non-zero = the state counts */
+    const int32_t *kv_lens;         /* nullable [B]: states 0 .. kv_lens[b]-1 count (clamped to 0 .. Lk) */
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    int64_t mask_stride[2];
+    int32_t B, Lq, Lk, Hq, Hk, D, dtype;
+    float scale;                    /* > 0 */
+} mvf_attn_desc;
+/* out [B,Lq,Hq,D] contiguous = softmax(scale q k^T over the states that count) v; zeros where none counts.
+ * States that do not count are never multiplied (their memory may hold anything).  lse (nullable, for the
+ * backward): B*Hq*Lq floats, [B,Hk,Lq,Hq/Hk].  workspace: ..._workspace_bytes(d), may be NULL when 0; 16-byte
+ * aligned, as out. */
+MVF_API size_t mvf_cross_attention_fwd_workspace_bytes(const mvf_attn_desc *d);
+MVF_API int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void *workspace, void *stream);
+/* out, lse from the forward, g_out [B,Lq,Hq,D]; g_q [B,Lq,Hq,D], g_k, g_v [B,Lk,Hk,D]: all contiguous and
+ * 16-byte aligned; g_k, g_v are zero where a state does not count, and may both be NULL.  No atomics:
+ * bit-reproducible. */
+MVF_API size_t mvf_cross_attention_bwd_workspace_bytes(const mvf_attn_desc *d);
+MVF_API int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float *lse, const void *g_out, void *g_q,
+                            void *g_k, void *g_v, void *workspace, void *stream);
+
+typedef struct mvf_qk_norm_desc {
+    const void *q, *k;              /* q [B,Lq,Hq,D], k [B,Lk,Hk,D]; k may be NULL (queries alone) */
+    const float *q_weight, *k_weight;   /* nullable [D] */
+    const void *q_pos, *k_pos;      /* nullable (no rotation) [L,axes] or [B,L,axes] contiguous int32 (int64: pos64) */
+    const uint64_t *freq;           /* HOST array of rot/(2 axes) fractions of a turn per unit of position, 2^64 = one turn */
+    int64_t q_stride[3], k_stride[3];
+    int64_t q_pos_stride, k_pos_stride; /* elements between the positions of two sequences, 0 = shared */
+    int32_t B, Lq, Lk, Hq, Hk, D, dtype, axes, rot, interleaved, pos64;
+    float eps;
+} mvf_qk_norm_desc;
+/* y = R(pos) (w * x * rsqrt(mean(x^2) + eps)) per head; the first `rot` channels are rotated, in `axes` equal
+ * blocks, pairs (2j, 2j+1) if interleaved, (j, j + block/2) otherwise.  Outputs contiguous, 16-byte aligned. */
+MVF_API int mvf_qk_norm_rope_fwd(const mvf_qk_norm_desc *d, void *q_out, void *k_out, void *stream);
+/* gradients of both; g_q_weight / g_k_weight nullable [D]; workspace: ..._workspace_floats(d).  No atomics. */
+MVF_API size_t mvf_qk_norm_rope_bwd_workspace_floats(const mvf_qk_norm_desc *d);
+MVF_API int mvf_qk_norm_rope_bwd(const mvf_qk_norm_desc *d, const void *g_q_out, const void *g_k_out, void *g_q, void *g_k,
+                         float *g_q_weight, float *g_k_weight, float *workspace, void *stream);
+
 /* ---- measurement hooks (bench.py) ------------------------------------------------------
  * When enabled, the library brackets launches of its kernels with a pair of HIP events recorded on the
  * launch stream.  mvf_profile_read() synchronises the recorded events and returns the summed kernel time
@@ -620,7 +669,11 @@ MVF_API int mvf_color_jitter(const float *img, const float *factors, const int32
 #define MVF_PROF_REGROUP_BWD 33      /* k_regroup_bwd */
 #define MVF_PROF_INTERLEAVE_FWD 34   /* k_interleave_fwd */
 #define MVF_PROF_SUM_ACT_FWD 35      /* k_sum_act_fwd */
-#define MVF_PROF_COUNT 36
+#define MVF_PROF_ATTN_FWD 36         /* k_attn_fwd (+ k_attn_join) */
+#define MVF_PROF_ATTN_BWD 37         /* k_attn_dq + k_attn_dkv (+ k_attn_sum) */
+#define MVF_PROF_QK_NORM_FWD 38      /* k_qk_norm_fwd */
+#define MVF_PROF_QK_NORM_BWD 39      /* k_qk_norm_bwd (+ k_qk_norm_dw) */
+#define MVF_PROF_COUNT 40
 /* launch tags of MVF_PROF_UNIT_FWDBWD (mvf_profile_read_launches): what kind of unit group a launch carried */
 #define MVF_TAG_SINGLE_FRAME 0  /* identity candidates evaluated (and possibly handed over: ident_out) */
 #define MVF_TAG_MULTI_FRAME 1   /* identity maps taken from another unit (ident_in) */

@@ -12,7 +12,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MVF_HOTPATH_LIB: developer knob (kernel variant builds); the product loads the in-tree library
 LIB_PATH = os.environ.get("MVF_HOTPATH_LIB") or os.path.join(_HERE, "lib", "libmvf_hotpath.so")
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 NO_SSIM, AVG_REPROJ, NO_AUTOMASK = 1, 2, 4
 MAX_SRC = 4
@@ -67,6 +67,28 @@ class SilogJob(C.Structure):
 
 
 MAX_SILOG_JOBS = 16
+
+DTYPE_F32, DTYPE_BF16 = 0, 1
+ATTN_MAX_D = 128
+
+
+class AttnDesc(C.Structure):
+    """mvf_attn_desc (include/mvf_hotpath.h)."""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("key_mask", _vp), ("kv_lens", _vp),
+        ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("mask_stride", _i64 * 2),
+        ("B", _i), ("Lq", _i), ("Lk", _i), ("Hq", _i), ("Hk", _i), ("D", _i), ("dtype", _i), ("scale", _f),
+    ]
+
+
+class QkNormDesc(C.Structure):
+    """mvf_qk_norm_desc (include/mvf_hotpath.h)."""
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp), ("q_pos", _vp), ("k_pos", _vp), ("freq", _vp),
+        ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("q_pos_stride", _i64), ("k_pos_stride", _i64),
+        ("B", _i), ("Lq", _i), ("Lk", _i), ("Hq", _i), ("Hk", _i), ("D", _i), ("dtype", _i), ("axes", _i), ("rot", _i),
+        ("interleaved", _i), ("pos64", _i), ("eps", _f),
+    ]
 
 # name -> argument ctypes (return type is always int = hipError_t unless listed in _RESTYPE)
 _SIGNATURES = {
@@ -169,6 +191,13 @@ _SIGNATURES = {
     "mvf_reflect_pad1_bwd": [_vp, _vp, _i, _i, _i, _vp],
     "mvf_affine_restore_fwd": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "mvf_affine_restore_bwd": [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
+    "mvf_cross_attention_fwd_workspace_bytes": [C.POINTER(AttnDesc)],
+    "mvf_cross_attention_fwd": [C.POINTER(AttnDesc), _vp, _vp, _vp, _vp],
+    "mvf_cross_attention_bwd_workspace_bytes": [C.POINTER(AttnDesc)],
+    "mvf_cross_attention_bwd": [C.POINTER(AttnDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "mvf_qk_norm_rope_fwd": [C.POINTER(QkNormDesc), _vp, _vp, _vp],
+    "mvf_qk_norm_rope_bwd_workspace_floats": [C.POINTER(QkNormDesc)],
+    "mvf_qk_norm_rope_bwd": [C.POINTER(QkNormDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     "mvf_profile_enable": [_i],
     "mvf_profile_reset": [],
     "mvf_profile_read": [_i, C.POINTER(C.c_double), C.POINTER(C.c_int64)],
@@ -178,7 +207,7 @@ _SIGNATURES = {
 }
 (PROF_UNIT_FWD, PROF_UNIT_BWD, PROF_PHOTO_FWD, PROF_PHOTO_BWD, PROF_WARP_FWD, PROF_WARP_BWD,
  PROF_UNIT_FWDBWD) = range(7)
-PROF_FIRST_GLUE, PROF_COUNT = 7, 36         # ids >= 7: glue kernels, profile level 2, work = algorithmic bytes
+PROF_FIRST_GLUE, PROF_COUNT = 7, 40         # ids >= 7: glue kernels, profile level 2, work = algorithmic bytes
 TAG_NAMES = {0: "single_frame", 1: "multi_frame", 2: "affine", 3: "single_frame+affine"}
 _RESTYPE = {"mvf_error_string": C.c_char_p, "mvf_profile_name": C.c_char_p, "mvf_profile_read_launches": C.c_int64, "mvf_workspace_floats": C.c_size_t,
             "mvf_flow_warp_workspace_floats": C.c_size_t, "mvf_fusion_prep_floats": C.c_size_t, "mvf_fusion_bwd_workspace_ints": C.c_size_t,
@@ -186,7 +215,9 @@ _RESTYPE = {"mvf_error_string": C.c_char_p, "mvf_profile_name": C.c_char_p, "mvf
             "mvf_up2cat_pad_act_workspace_floats": C.c_size_t, "mvf_fusion_lists_level_ints": C.c_size_t, "mvf_fusion_lists_scratch_ints": C.c_size_t,
             "mvf_color_jitter_workspace_floats": C.c_size_t, "mvf_bias_act_workspace_floats": C.c_size_t,
             "mvf_units_workspace_floats": C.c_size_t, "mvf_units_ticket_ints": C.c_size_t,
-            "mvf_resize_bilinear_bwd_workspace_floats": C.c_size_t}
+            "mvf_resize_bilinear_bwd_workspace_floats": C.c_size_t,
+            "mvf_cross_attention_fwd_workspace_bytes": C.c_size_t, "mvf_cross_attention_bwd_workspace_bytes": C.c_size_t,
+            "mvf_qk_norm_rope_bwd_workspace_floats": C.c_size_t}
 
 EXPORTS = tuple(_SIGNATURES)
 

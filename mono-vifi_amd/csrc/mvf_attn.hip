@@ -1,0 +1,824 @@
+// mvf_attn.hip -- cross attention of the tokens of one frame to the tokens of others: forward and backward.
+//
+//     o[b,i,h] = sum_j P[i,j] v[b,j,h/G],  P[i,:] = softmax_j(scale * q[b,i,h] . k[b,j,h/G]) over the states j that count
+//
+// with G = Hq / Hk query heads reading one head of keys and values, kv_lens[b] states per sequence and a byte mask of
+// states.  A state that does not count contributes nothing whatever its memory holds (it is staged as zeros, its score is
+// -inf); a query no state counts for gets zeros, and zero gradients.
+//
+// The scores never reach memory.  A wave owns 32 query rows (row r = i * G + g: the G heads that share a head of keys are
+// rows of the same tile, so one staged tile serves them all) and walks the states in tiles, keeping the running maximum m,
+// the sum l and the output tile in registers:
+//     S^T = K Q^T (32 x 32 x 16 matrix instructions: a lane holds ONE query, 16 of the 32 states of a tile),
+//     m' = max(m, max S), P^T = exp2(c S^T - c m'), l' = l exp2(c m - c m') + sum P,  O^T = O^T exp2(c m - c m') + V^T P^T
+// with c = scale * log2(e).  Computing the TRANSPOSED products keeps the softmax of a query inside two lanes (lane, lane ^ 32)
+// and makes the accumulator of S^T directly the right operand of V^T P^T: the order in which a lane holds the states of a
+// tile is a permutation of the reduction index, and V is read from LDS in the same permutation (ds_read_b64_tr_b16: four
+// states of one channel per lane), so P never moves between lanes.
+//
+// Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane.  fp32 inputs are three
+// (x = x0 + x1 + x2, each the leading 8 significand bits of what the previous left: exact), a product the six terms of
+// order <= 2: relative error ~2^-23 per product, and still 2.6 x the rate of the fp32 matrix instructions (6 x 32 cycles
+// against 8 x 64 for a 32 x 32 x 16 product).
+//
+// Compiled without contraction (the library's flag); fused multiply-adds are written out.
+#include "mvf_common.hpp"
+
+using namespace mvf;
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int NT = 256;            // four waves
+constexpr int PADE = 8;            // bf16 elements appended to an LDS row: 16-byte row reads of 16 lanes hit 64 different banks
+constexpr float kLog2e = 1.4426950408889634f;
+
+#define LDS_PTR(T) __attribute__((address_space(3))) T *
+
+// ------------------------------------------------------------------------------------------------- planes
+template <int NP>
+struct Frag {
+    bf16x8 p[NP];
+};
+template <int NP>
+struct Elem;
+template <>
+struct Elem<1> {
+    typedef __bf16 T;
+};
+template <>
+struct Elem<3> {
+    typedef float T;
+};
+
+MVF_DEV float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+MVF_DEV short top16(float x) { return (short)(__float_as_uint(x) >> 16); }
+
+// eight fp32 values -> NP planes of bf16.  One plane rounds to nearest even (half a step, 2^-8 of the value); three planes
+// cut, so that every remainder is exact.  (An infinity stays in plane 0 and leaves no remainder: what it multiplies becomes
+// infinite, or NaN where the other factor has an empty plane.)
+template <int NP>
+MVF_DEV Frag<NP> split8(const float (&x)[8])
+{
+    Frag<NP> f;
+    if constexpr (NP == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f.p[0][e] = (__bf16)x[e];
+    } else {
+        s16x8 a, b, c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float hi = trunc_bf16(x[e]);
+            const float r1 = __builtin_isinf(hi) ? 0.0f : x[e] - hi;
+            const float mid = trunc_bf16(r1);
+            a[e] = top16(hi);
+            b[e] = top16(mid);
+            c[e] = top16(r1 - mid);
+        }
+        f.p[0] = __builtin_bit_cast(bf16x8, a);
+        f.p[1] = __builtin_bit_cast(bf16x8, b);
+        f.p[2] = __builtin_bit_cast(bf16x8, c);
+    }
+    return f;
+}
+
+// c += a b; the small terms of the three-plane product first
+template <int NP>
+MVF_DEV f32x16 mma(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
+{
+    if constexpr (NP == 3) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    }
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
+// channels d0 .. d0 + 7 of a row of D channels (zeros behind D); `wide`: rows are 16-byte aligned and D a multiple of 8
+MVF_DEV void load8(const float *row, int d0, int D, bool wide, float (&x)[8])
+{
+    if (wide && d0 < D) {
+        const f32x4 a = *(const f32x4 *)(row + d0), b = *(const f32x4 *)(row + d0 + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = d0 + e < D ? row[d0 + e] : 0.0f;
+}
+template <int NP>
+MVF_DEV Frag<NP> load_frag(const typename Elem<NP>::T *row, int d0, int D, bool wide, bool live)
+{
+    Frag<NP> f;
+    if constexpr (NP == 1) {
+        if (live && wide && d0 < D) {
+            f.p[0] = *(const bf16x8 *)(row + d0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f.p[0][e] = (live && d0 + e < D) ? row[d0 + e] : (__bf16)0.0f;
+        }
+        return f;
+    } else {
+        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (live) load8(row, d0, D, wide, x);
+        return split8<NP>(x);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- LDS tiles
+// a tile of ROWS x DP values: NP planes of [ROWS][DP + PADE] bf16
+template <int NP, int ROWS, int DP>
+struct Tile {
+    static constexpr int LD = DP + PADE, PLANE = ROWS * LD, CHUNKS = ROWS * (DP / 8);
+    short v[NP * PLANE];
+
+    // one 8-channel chunk
+    MVF_DEV void put(int row, int chunk, const Frag<NP> &f)
+    {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *(bf16x8 *)&v[p * PLANE + row * LD + chunk * 8] = f.p[p];
+    }
+    // left operand whose rows are the tile's rows, reduced over 16 channels: row r0 + (lane & 31), channels k0 + 8 (lane >> 5) + e
+    MVF_DEV Frag<NP> rows(int r0, int k0, int lane) const
+    {
+        Frag<NP> f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) f.p[p] = *(const bf16x8 *)&v[p * PLANE + (r0 + (lane & 31)) * LD + k0 + 8 * (lane >> 5)];
+        return f;
+    }
+    // left operand whose rows are channels d0 + (lane & 31), reduced over the 16 rows r0 .. r0 + 15 in the order an
+    // accumulator holds them: element e of lane half h is row r0 + 4h + (e & 3) + 8 (e >> 2).  The transposing read hands
+    // lane t of a group of 16 the four rows of column t; lane t supplies the address of row t / 4, columns 4 (t & 3) ..
+    MVF_DEV Frag<NP> cols(int d0, int r0, int lane) const
+    {
+        const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2), col = d0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        Frag<NP> f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const short *a = &v[p * PLANE + row * LD + col];
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))a);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(a + 8 * LD));
+            s16x8 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[e] = lo[e]; x[4 + e] = hi[e]; }
+            f.p[p] = __builtin_bit_cast(bf16x8, x);
+        }
+        return f;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------- arguments
+struct AttnArgs {
+    const void *q, *k, *v, *o, *go;
+    void *out, *dq, *dk, *dv;
+    float *lse, *delta, *part, *part2;
+    const uint8_t *mask;
+    const int32_t *lens;
+    int64_t qs[3], ks[3], vs[3], ms[2];       // batch, token, head strides in elements; mask: batch, state
+    int B, Lq, Lk, Hq, Hk, D, G, R;           // R = Lq * G rows per (batch, key head)
+    int tiles, splits, per;                   // row or state tiles of a block row, parts of the reduction, reduction tiles per part
+    int wide;
+    float scale, c;                           // c = scale * log2(e)
+};
+
+// Consecutive workgroups go to consecutive XCDs, whose L2s do not share: give every XCD one contiguous run of the
+// (sequence, head)-major order, so that the tiles that read the same keys and values find them in one L2.
+MVF_DEV int xcd_run(int bid, int n)
+{
+    const int q = n >> 3, r = n & 7, x = bid & 7, y = bid >> 3;
+    return x * q + min(x, r) + y;
+}
+
+MVF_DEV int64_t row_off(const int64_t (&s)[3], int b, int r, int hk, int G)
+{
+    const int i = G == 1 ? r : r / G, g = G == 1 ? 0 : r - i * G;
+    return (int64_t)b * s[0] + (int64_t)i * s[1] + (int64_t)(hk * G + g) * s[2];
+}
+MVF_DEV int64_t dense_row(int b, int r, int hk, const AttnArgs &a)       // row of a contiguous [B, Lq, Hq, D]
+{
+    const int i = a.G == 1 ? r : r / a.G, g = a.G == 1 ? 0 : r - i * a.G;
+    return (((int64_t)b * a.Lq + i) * a.Hq + hk * a.G + g) * a.D;
+}
+MVF_DEV int states_of(const AttnArgs &a, int b)
+{
+    return a.lens ? max(0, min(a.lens[b], a.Lk)) : a.Lk;
+}
+// which of the 64 states from j0 on count, as a bit each (the same in every lane)
+MVF_DEV uint64_t live_states(const AttnArgs &a, int b, int j0, int n, int lane)
+{
+    const int j = j0 + lane;
+    bool ok = j < n;
+    if (ok && a.mask) ok = a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0;
+    return __ballot(ok);
+}
+
+// tile <- rows j0 .. of the states (or query rows) through `row_ptr(row)`; rows that do not count become zeros
+template <int NP, int ROWS, int DP, typename F>
+MVF_DEV void stage(Tile<NP, ROWS, DP> &t, const AttnArgs &a, F row_ptr)
+{
+    constexpr int CPR = DP / 8;
+#pragma unroll
+    for (int c0 = 0; c0 < Tile<NP, ROWS, DP>::CHUNKS; c0 += NT) {
+        const int c = c0 + threadIdx.x;
+        if ((Tile<NP, ROWS, DP>::CHUNKS % NT) && c >= Tile<NP, ROWS, DP>::CHUNKS) break;
+        const int row = c / CPR, ch = c - row * CPR;
+        const typename Elem<NP>::T *p = row_ptr(row);
+        t.put(row, ch, load_frag<NP>(p, ch * 8, a.D, a.wide, p != nullptr));
+    }
+}
+
+MVF_DEV float other_half_max(float x)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+MVF_DEV float other_half_sum(float x)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// state (or row) of accumulator element r of lane half h within a 32-tile
+MVF_DEV constexpr int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// elements 8 s .. 8 s + 7 of an accumulator as the right operand of a product reduced over the rows r0 = 16 s .. of the tile
+template <int NP>
+MVF_DEV Frag<NP> acc_frag(const f32x16 &x, int s)
+{
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
+    return split8<NP>(y);
+}
+
+// four consecutive channels d .. d + 3 of a row
+MVF_DEV void store4(float *row, int d, int D, bool wide, float a, float b, float c, float e)
+{
+    if (wide && d < D) { *(f32x4 *)(row + d) = f32x4{a, b, c, e}; return; }
+    const float x[4] = {a, b, c, e};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (d + i < D) row[d + i] = x[i];
+}
+MVF_DEV void store4(__bf16 *row, int d, int D, bool wide, float a, float b, float c, float e)
+{
+    const float x[4] = {a, b, c, e};
+    if (wide && d < D) {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        bf16x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = (__bf16)x[i];
+        *(bf16x4 *)(row + d) = y;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (d + i < D) row[d + i] = (__bf16)x[i];
+}
+// accumulator tiles (channel rows, this lane's column) -> a row of D channels, scaled
+template <int DT, typename T>
+MVF_DEV void store_cols(T *row, const f32x16 (&acc)[DT], float f, int D, bool wide, int h)
+{
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            store4(row, 32 * t + 8 * i + 4 * h, D, wide, acc[t][4 * i] * f, acc[t][4 * i + 1] * f, acc[t][4 * i + 2] * f,
+                   acc[t][4 * i + 3] * f);
+}
+
+// ------------------------------------------------------------------------------------------------- forward
+// grid: (batch x key head) major, then the part of the states, then the row tile (128 rows)
+template <int NP, int DP, int BK>
+__global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
+{
+    typedef typename Elem<NP>::T T;
+    constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tk;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    int id = xcd_run(blockIdx.x, gridDim.x);
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int r = tile * 128 + wave * 32 + col;
+    const bool live = r < a.R;
+    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
+    Frag<NP> qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, a.wide, live);
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const int n = states_of(a, b);
+    const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
+    const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
+    const int j1 = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * BK);
+    for (int j0 = part * a.per * BK; j0 < j1; j0 += BK) {
+        uint64_t bits = live_states(a, b, j0, n, lane);
+        if (BK < 64) bits &= (1ull << (BK & 63)) - 1;
+        if (bits == 0) continue;
+        __syncthreads();
+        stage(tk, a, [&](int row) { return (bits >> row) & 1 ? kb + (int64_t)(j0 + row) * a.ks[1] : (const T *)nullptr; });
+        stage(tv, a, [&](int row) { return (bits >> row) & 1 ? vb + (int64_t)(j0 + row) * a.vs[1] : (const T *)nullptr; });
+        __syncthreads();
+        f32x16 s[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < KS; ++x) s[t] = mma(tk.rows(32 * t, 16 * x, lane), qf[x], s[t]);
+        }
+        const uint64_t full = BK < 64 ? (1ull << (BK & 63)) - 1 : ~0ull;
+        if (bits != full) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const uint32_t w = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!((w >> acc_row(i, 0)) & 1)) s[t][i] = -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = fmaxf(m, other_half_max(mx));
+        const float mc = (mx == -INFINITY ? 0.0f : mx) * a.c;
+        const float f = __builtin_amdgcn_exp2f(fmaf(m, a.c, -mc));
+        m = mx;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] *= f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.c, -mc));
+                l += p;
+                s[t][i] = p;
+            }
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const Frag<NP> p = acc_frag<NP>(s[t], x);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] = mma(tv.cols(32 * d, 32 * t + 16 * x, lane), p, o[d]);
+            }
+    }
+    l = other_half_sum(l);
+    if (!live) return;
+    if (a.splits > 1) {                                          // this part's maximum, sum and unscaled output
+        const int64_t w = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+        store_cols<DT>(a.part + w * a.D, o, 1.0f, a.D, (a.D & 3) == 0, h);
+        if (h == 0) {
+            a.part2[2 * w] = m * a.c;
+            a.part2[2 * w + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, (a.D & 7) == 0, h);
+    if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l));
+}
+
+// joins the parts of a row: o = sum_p o_p 2^(m_p - m) / sum_p l_p 2^(m_p - m).  One lane per four channels.
+template <typename T>
+__global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a)
+{
+    const int per = (a.D + 3) / 4;
+    const int64_t idx = (int64_t)blockIdx.x * NT + threadIdx.x, rows = (int64_t)a.B * a.Hk * a.R;
+    const int64_t w = idx / per;
+    if (w >= rows) return;
+    const int d = (int)(idx - w * per) * 4;
+    float m = -INFINITY;
+    for (int p = 0; p < a.splits; ++p) {
+        const int64_t y = p * rows + w;
+        if (a.part2[2 * y + 1] != 0.0f) m = fmaxf(m, a.part2[2 * y]);
+    }
+    float l = 0.0f, o[4] = {0, 0, 0, 0};
+    for (int p = 0; p < a.splits; ++p) {
+        const int64_t y = p * rows + w;
+        const float lp = a.part2[2 * y + 1];
+        if (lp == 0.0f) continue;                                // nothing counted in this part
+        const float f = __builtin_amdgcn_exp2f(a.part2[2 * y] - m);
+        l = fmaf(lp, f, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < a.D) o[i] = fmaf(a.part[y * a.D + d + i], f, o[i]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int bh = (int)(w / a.R), r = (int)(w - (int64_t)bh * a.R), b = bh / a.Hk, hk = bh - b * a.Hk;
+    store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 7) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (a.lse && d == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// ------------------------------------------------------------------------------------------------- backward
+// P is recomputed from the stored log2 of the softmax sum; delta = do . o is what the softmax subtracts from dP:
+//     dS = P (dP - delta),  dP = do V^T,  dq = scale dS K,  dk = scale dS^T q,  dv = P^T do
+// Two passes without atomics, so that the sums have one order: rows own dq (and write delta), states own dk and dv.  The
+// heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
+
+// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
+template <int NP, int DP, int BK>
+__global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
+{
+    typedef typename Elem<NP>::T T;
+    constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tk;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    int id = xcd_run(blockIdx.x, gridDim.x);
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int r = tile * 128 + wave * 32 + col;
+    const bool live = r < a.R;
+    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
+    const int64_t dense = live ? dense_row(b, r, hk, a) : 0;
+    const bool dwide = (a.D & 7) == 0;
+    Frag<NP> qf[KS], gf[KS];
+    float delta = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, a.wide, live);
+        gf[s] = load_frag<NP>((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
+        const T *orow = (const T *)a.o + dense, *grow = (const T *)a.go + dense;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = 16 * s + 8 * h + e;
+            if (live && d < a.D) delta = fmaf((float)grow[d], (float)orow[d], delta);
+        }
+    }
+    delta = other_half_sum(delta);
+    const float lse = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
+    if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta;
+    f32x16 dq[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[t][i] = 0.0f;
+    const int n = states_of(a, b);
+    const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
+    const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
+    const int j1 = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * BK);
+    for (int j0 = part * a.per * BK; j0 < j1; j0 += BK) {
+        uint64_t bits = live_states(a, b, j0, n, lane);
+        if (BK < 64) bits &= (1ull << (BK & 63)) - 1;
+        if (bits == 0) continue;
+        __syncthreads();
+        stage(tk, a, [&](int row) { return (bits >> row) & 1 ? kb + (int64_t)(j0 + row) * a.ks[1] : (const T *)nullptr; });
+        stage(tv, a, [&](int row) { return (bits >> row) & 1 ? vb + (int64_t)(j0 + row) * a.vs[1] : (const T *)nullptr; });
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+                s = mma(tk.rows(32 * t, 16 * x, lane), qf[x], s);
+                dp = mma(tv.rows(32 * t, 16 * x, lane), gf[x], dp);
+            }
+            // a state that does not count: its row of the tile is zero, so whatever dS holds for it adds nothing to dq --
+            // but exp2(-lse) may be infinite there, so it is cleared
+            const uint32_t w = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = (w >> acc_row(i, 0)) & 1 ? __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) : 0.0f;
+                s[i] = p * (dp[i] - delta);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const Frag<NP> ds = acc_frag<NP>(s, x);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) dq[d] = mma(tk.cols(32 * d, 32 * t + 16 * x, lane), ds, dq[d]);
+            }
+        }
+    }
+    if (!live) return;
+    if (a.splits > 1) {
+        const int64_t w = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+        store_cols<DT>(a.part + w * a.D, dq, a.scale, a.D, (a.D & 3) == 0, h);
+        return;
+    }
+    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, dwide, h);
+}
+
+// grid: (batch x key head) major, then the part of the rows, then the state tile (128 states, 32 per wave).  Row tiles of q and
+// do are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS
+template <int NP, int DP, int BQ>
+__global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
+{
+    typedef typename Elem<NP>::T T;
+    constexpr int KS = DP / 16, DT = DP / 32, QT = BQ / 32;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BQ, DP> tq;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BQ, DP> tg;
+    __shared__ __attribute__((aligned(16))) float sl[BQ], sd[BQ];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    int id = xcd_run(blockIdx.x, gridDim.x);
+    const int tile = id % a.tiles;
+    id /= a.tiles;
+    const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
+    const int j = tile * 128 + wave * 32 + col;
+    const int n = states_of(a, b);
+    const bool mine = j < a.Lk;
+    bool live = j < n;
+    if (live && a.mask) live = a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0;
+    const T *krow = (const T *)a.k + (live ? (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)hk * a.ks[2] : 0);
+    const T *vrow = (const T *)a.v + (live ? (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)hk * a.vs[2] : 0);
+    Frag<NP> kf[KS], vf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        kf[s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, a.wide, live);
+        vf[s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, a.wide, live);
+    }
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.0f;
+    const int r1 = (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ);
+    const bool any = tile * 128 < n;                              // (the same in every lane of the workgroup)
+    for (int r0 = part * a.per * BQ; any && r0 < r1; r0 += BQ) {
+        __syncthreads();
+        stage(tq, a, [&](int row) { return r0 + row < a.R ? (const T *)a.q + row_off(a.qs, b, r0 + row, hk, a.G) : (const T *)nullptr; });
+        stage(tg, a, [&](int row) { return r0 + row < a.R ? (const T *)a.go + dense_row(b, r0 + row, hk, a) : (const T *)nullptr; });
+        if (threadIdx.x < BQ) {
+            const int r = r0 + threadIdx.x;
+            sl[threadIdx.x] = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;      // rows behind the last: P = 0
+            sd[threadIdx.x] = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < KS; ++x) {
+                s = mma(tq.rows(32 * t, 16 * x, lane), kf[x], s);
+                dp = mma(tg.rows(32 * t, 16 * x, lane), vf[x], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 ls = *(const f32x4 *)&sl[32 * t + acc_row(4 * i, h)], de = *(const f32x4 *)&sd[32 * t + acc_row(4 * i, h)];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = live ? __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], a.c, -ls[e])) : 0.0f;
+                    s[4 * i + e] = p;
+                    dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const Frag<NP> p = acc_frag<NP>(s, x), ds = acc_frag<NP>(dp, x);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    dv[d] = mma(tg.cols(32 * d, 32 * t + 16 * x, lane), p, dv[d]);
+                    dk[d] = mma(tq.cols(32 * d, 32 * t + 16 * x, lane), ds, dk[d]);
+                }
+            }
+        }
+    }
+    if (!mine) return;
+    if (a.splits > 1) {
+        const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, w = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
+        const bool pw = (a.D & 3) == 0;
+        store_cols<DT>(a.part + w, dk, live ? a.scale : 0.0f, a.D, pw, h);
+        store_cols<DT>(a.part + w + n1, dv, 1.0f, a.D, pw, h);
+        return;
+    }
+    const int64_t w = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
+    store_cols<DT>((T *)a.dk + w, dk, a.scale, a.D, (a.D & 7) == 0, h);
+    store_cols<DT>((T *)a.dv + w, dv, 1.0f, a.D, (a.D & 7) == 0, h);
+}
+
+// adds the parts of a gradient, in order.  KV: part[p][2][B * Hk][Lk][D] -> dk, dv [B, Lk, Hk, D]; otherwise part[p][B * Hk][R][D] -> dq
+template <typename T, bool KV>
+__global__ void __launch_bounds__(NT) k_attn_sum(const AttnArgs a)
+{
+    const int per = (a.D + 3) / 4, len = KV ? a.Lk : a.R;
+    const int64_t idx = (int64_t)blockIdx.x * NT + threadIdx.x, rows = (int64_t)a.B * a.Hk * len;
+    int64_t w = idx / per;
+    const int d = (int)(idx - w * per) * 4;
+    const int which = KV && w >= rows;
+    if (which) w -= rows;
+    if (w >= rows) return;
+    float x[4] = {0, 0, 0, 0};
+    for (int p = 0; p < a.splits; ++p) {
+        const float *y = a.part + (((KV ? 2 * p + which : p) * rows) + w) * a.D + d;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < a.D) x[i] += y[i];
+    }
+    const int bh = (int)(w / len), r = (int)(w - (int64_t)bh * len), b = bh / a.Hk, hk = bh - b * a.Hk;
+    T *dst = KV ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D : (T *)a.dq + dense_row(b, r, hk, a);
+    store4(dst, d, a.D, (a.D & 7) == 0, x[0], x[1], x[2], x[3]);
+}
+
+// ------------------------------------------------------------------------------------------------- host side
+constexpr int kWant = 512;         // workgroups that fill the chip (two per CU)
+
+// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: enough to fill the chip, at least
+// four tiles each, at most 64
+void split_of(int64_t blocks, int red, int &splits, int &per)
+{
+    int64_t s = blocks > 0 ? (kWant + blocks - 1) / blocks : 1;
+    s = s > 64 ? 64 : s;
+    const int most = red / 4 > 1 ? red / 4 : 1;
+    if (s > most) s = most;
+    per = s > 0 ? (int)((red + s - 1) / s) : red;
+    if (per < 1) per = 1;
+    splits = red > 0 ? (red + per - 1) / per : 1;
+}
+
+struct Plan {
+    int NP, DP, BK, BQ;
+    int rtiles, ktiles;                      // 128-row tiles, 128-state tiles
+    int fs, fper, qs, qper, ks, kper;        // forward, dq, dkv
+};
+Plan plan_of(const mvf_attn_desc &d)
+{
+    Plan p;
+    p.NP = d.dtype == MVF_DTYPE_F32 ? 3 : 1;
+    p.DP = d.D <= 32 ? 32 : d.D <= 64 ? 64 : d.D <= 96 ? 96 : 128;
+    p.BK = p.NP == 1 ? 64 : 32;
+    p.BQ = 32;
+    const int R = d.Lq * (d.Hq / d.Hk);
+    p.rtiles = (R + 127) / 128;
+    p.ktiles = (d.Lk + 127) / 128;
+    const int64_t bh = (int64_t)d.B * d.Hk;
+    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
+    p.qs = p.fs;
+    p.qper = p.fper;
+    split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, p.ks, p.kper);
+    return p;
+}
+bool bad_desc(const mvf_attn_desc *d)
+{
+    if (!d || d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->Hq <= 0 || d->Hk <= 0 || d->Hq % d->Hk || d->D <= 0 || d->D > MVF_ATTN_MAX_D) return true;
+    if (d->dtype != MVF_DTYPE_F32 && d->dtype != MVF_DTYPE_BF16) return true;
+    if (!(d->scale > 0.0f) || !(d->scale * kLog2e < INFINITY)) return true;
+    const int64_t G = d->Hq / d->Hk, R = G * d->Lq, bh = (int64_t)d->B * d->Hk;
+    // 32-bit tile and workgroup counts (offsets into the tensors are 64-bit throughout)
+    if (R > (1 << 30) || d->Lk > (1 << 30) || bh * ((R + 127) / 128 + (d->Lk + 127) / 128 + 1) * 64 > 0x7fffffffLL) return true;
+    return false;
+}
+int64_t elem_blocks(int64_t n) { return (n + NT - 1) / NT; }
+
+AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
+{
+    AttnArgs a = {};
+    a.q = d.q; a.k = d.k; a.v = d.v;
+    a.mask = d.key_mask; a.lens = d.kv_lens;
+    bool wide = d.D % 8 == 0;
+    const int64_t align = p.NP == 1 ? 8 : 4;             // elements in 16 bytes
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i];
+        wide = wide && a.qs[i] % align == 0 && a.ks[i] % align == 0 && a.vs[i] % align == 0;
+    }
+    wide = wide && !(((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) & 15);
+    a.wide = wide;
+    a.ms[0] = d.mask_stride[0]; a.ms[1] = d.mask_stride[1];
+    a.B = d.B; a.Lq = d.Lq; a.Lk = d.Lk; a.Hq = d.Hq; a.Hk = d.Hk; a.D = d.D;
+    a.G = d.Hq / d.Hk;
+    a.R = d.Lq * a.G;
+    a.scale = d.scale;
+    a.c = d.scale * kLog2e;
+    return a;
+}
+
+template <int NP, int DP>
+void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_attn_fwd<NP, DP, NP == 1 ? 64 : 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+}
+template <int NP, int DP>
+void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_attn_dq<NP, DP, NP == 1 ? 64 : 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+}
+template <int NP, int DP>
+void launch_dkv(const AttnArgs &a, int64_t blocks, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+}
+#define MVF_ATTN_PICK(fn, p, ...)                                                                      \
+    do {                                                                                               \
+        if ((p).NP == 1) {                                                                             \
+            if ((p).DP == 32) fn<1, 32>(__VA_ARGS__);                                                  \
+            else if ((p).DP == 64) fn<1, 64>(__VA_ARGS__);                                             \
+            else if ((p).DP == 96) fn<1, 96>(__VA_ARGS__);                                             \
+            else fn<1, 128>(__VA_ARGS__);                                                              \
+        } else {                                                                                       \
+            if ((p).DP == 32) fn<3, 32>(__VA_ARGS__);                                                  \
+            else if ((p).DP == 64) fn<3, 64>(__VA_ARGS__);                                             \
+            else if ((p).DP == 96) fn<3, 96>(__VA_ARGS__);                                             \
+            else fn<3, 128>(__VA_ARGS__);                                                              \
+        }                                                                                              \
+    } while (0)
+
+int64_t tensor_bytes(const mvf_attn_desc &d, int64_t rows) { return rows * d.D * (d.dtype == MVF_DTYPE_F32 ? 4 : 2); }
+
+}  // namespace
+
+extern "C" {
+
+size_t mvf_cross_attention_fwd_workspace_bytes(const mvf_attn_desc *d)
+{
+    if (bad_desc(d)) return 0;
+    const Plan p = plan_of(*d);
+    const int64_t rows = (int64_t)d->B * d->Hq * d->Lq;
+    return p.fs > 1 ? (size_t)(p.fs * rows * (d->D + 2) * 4) : 0;
+}
+
+int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void *workspace, void *stream)
+{
+    if (bad_desc(d)) return (int)hipErrorInvalidValue;
+    if (d->B == 0 || d->Lq == 0) return 0;
+    const Plan p = plan_of(*d);
+    if (!d->q || !out || (d->Lk > 0 && (!d->k || !d->v)) || (p.fs > 1 && !workspace) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 15))
+        return (int)hipErrorInvalidValue;
+    AttnArgs a = args_of(*d, p);
+    const int64_t rows = (int64_t)d->B * d->Hq * d->Lq;
+    a.out = out;
+    a.lse = lse;
+    a.tiles = p.rtiles; a.splits = p.fs; a.per = p.fper;
+    a.part = (float *)workspace;
+    a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
+    MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
+    if (p.fs > 1) {
+        const int64_t nb = elem_blocks(rows * ((d->D + 3) / 4));
+        if (p.NP == 1) hipLaunchKernelGGL(k_attn_join<__bf16>, dim3((unsigned)nb), dim3(NT), 0, st, a);
+        else hipLaunchKernelGGL(k_attn_join<float>, dim3((unsigned)nb), dim3(NT), 0, st, a);
+    }
+    return hip_check_launch();
+}
+
+size_t mvf_cross_attention_bwd_workspace_bytes(const mvf_attn_desc *d)
+{
+    if (bad_desc(d)) return 0;
+    const Plan p = plan_of(*d);
+    const int64_t rows = (int64_t)d->B * d->Hq * d->Lq, states = (int64_t)d->B * d->Hk * d->Lk;
+    const int64_t delta = (rows + 3) / 4 * 4;
+    const int64_t pq = p.qs > 1 ? p.qs * rows * d->D : 0, pk = p.ks > 1 ? 2 * p.ks * states * d->D : 0;
+    return (size_t)((delta + (pq > pk ? pq : pk)) * 4);
+}
+
+int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float *lse, const void *g_out, void *g_q, void *g_k,
+                            void *g_v, void *workspace, void *stream)
+{
+    if (bad_desc(d)) return (int)hipErrorInvalidValue;
+    if (d->B == 0) return 0;
+    if (d->Lq > 0 && (!d->q || !out || !lse || !g_out || !g_q || !workspace)) return (int)hipErrorInvalidValue;
+    if (d->Lk > 0 && (!d->k || !d->v || !g_k != !g_v)) return (int)hipErrorInvalidValue;
+    if (((uintptr_t)out | (uintptr_t)g_out | (uintptr_t)g_q | (uintptr_t)g_k | (uintptr_t)g_v | (uintptr_t)workspace) & 15)
+        return (int)hipErrorInvalidValue;
+    const Plan p = plan_of(*d);
+    AttnArgs a = args_of(*d, p);
+    const int64_t rows = (int64_t)d->B * d->Hq * d->Lq, states = (int64_t)d->B * d->Hk * d->Lk;
+    a.o = out; a.go = g_out; a.lse = const_cast<float *>(lse);
+    a.dq = g_q; a.dk = g_k; a.dv = g_v;
+    a.delta = (float *)workspace;
+    a.part = a.delta + (rows + 3) / 4 * 4;
+    hipStream_t st = (hipStream_t)stream;
+    ProfScope ps(MVF_PROF_ATTN_BWD, st, tensor_bytes(*d, 4 * rows + 4 * states));
+    if (d->Lq > 0) {
+        a.tiles = p.rtiles; a.splits = p.qs; a.per = p.qper;
+        MVF_ATTN_PICK(launch_dq, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.qs, st);
+        if (p.qs > 1) {
+            const int64_t nb = elem_blocks(rows * ((d->D + 3) / 4));
+            if (p.NP == 1) hipLaunchKernelGGL((k_attn_sum<__bf16, false>), dim3((unsigned)nb), dim3(NT), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_sum<float, false>), dim3((unsigned)nb), dim3(NT), 0, st, a);
+        }
+    }
+    if (d->Lk > 0 && g_k) {
+        a.tiles = p.ktiles; a.splits = p.ks; a.per = p.kper;
+        MVF_ATTN_PICK(launch_dkv, p, a, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
+        if (p.ks > 1) {
+            const int64_t nb = elem_blocks(2 * states * ((d->D + 3) / 4));
+            if (p.NP == 1) hipLaunchKernelGGL((k_attn_sum<__bf16, true>), dim3((unsigned)nb), dim3(NT), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_sum<float, true>), dim3((unsigned)nb), dim3(NT), 0, st, a);
+        }
+    }
+    return hip_check_launch();
+}
+
+}  // extern "C"

@@ -9,6 +9,8 @@ surrounding MIOpen kernels and with DDP's reducer through normal stream semantic
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 
 import numpy as np
 import torch
@@ -1878,3 +1880,236 @@ def color_jitter(img, factors, order, apply, flip, frames=1, want_raw=False):
                                          nat.ptr(flip), nat.ptr(raw), nat.ptr(aug), nat.ptr(ws), S, frames, H, W,
                                          _stream()), "color_jitter")
     return raw, aug
+
+
+# ------------------------------------------------------------------ token attention
+_ATTN_TYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
+
+
+def _token_heads(what, name, t, dtype=None):
+    """[batch, token, head, channel] with adjacent channels, float32 or bfloat16; any strides otherwise."""
+    if not torch.is_tensor(t) or t.dim() != 4:
+        raise RuntimeError(f"{what}: {name} must be [batch, tokens, heads, channels], got "
+                           f"{tuple(t.shape) if torch.is_tensor(t) else type(t).__name__}")
+    if t.dtype not in _ATTN_TYPES:
+        raise RuntimeError(f"{what}: {name} must be float32 or bfloat16, got {t.dtype}")
+    if dtype is not None and t.dtype != dtype:
+        raise RuntimeError(f"{what}: {name} is {t.dtype}, the queries are {dtype}")
+    H, D = t.shape[2:]
+    if H < 1 or D < 1 or D > nat.ATTN_MAX_D:
+        raise RuntimeError(f"{what}: {name} needs at least one head of 1..{nat.ATTN_MAX_D} channels, got {tuple(t.shape)}")
+    return t if D == 1 or t.stride(3) == 1 else t.contiguous()
+
+
+def _once(what):
+    # (torch's once_differentiable looks at the incoming gradient alone: a second derivative through the saved inputs would
+    # be silently missing)
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once: its backward does not run under create_graph=True")
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+class CrossAttention(torch.autograd.Function):
+    """softmax(scale q k^T) v over the states that count (csrc/mvf_attn.hip).  No counterpart in the reference, whose fusion of
+    neighbour frames is a warp and a mask (networks/fusion_module.py:100-130)."""
+
+    @staticmethod
+    def _desc(q, k, v, key_mask, kv_lens, scale):
+        B, Lq, Hq, D = q.shape
+        d = nat.AttnDesc(q=_addr(q), k=_addr(k), v=_addr(v), key_mask=_addr(key_mask), kv_lens=_addr(kv_lens), B=B, Lq=Lq,
+                         Lk=k.shape[1], Hq=Hq, Hk=k.shape[2], D=D, dtype=_ATTN_TYPES[q.dtype], scale=scale)
+        d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        if key_mask is not None:
+            d.mask_stride[:] = key_mask.stride()
+        return d
+
+    @staticmethod
+    def forward(ctx, q, k, v, key_mask, kv_lens, scale):
+        lib = nat.lib()
+        d = CrossAttention._desc(q, k, v, key_mask, kv_lens, scale)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        grad = any(ctx.needs_input_grad[:3])
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if grad else None
+        n = lib.mvf_cross_attention_fwd_workspace_bytes(C.byref(d))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        nat.check(lib.mvf_cross_attention_fwd(C.byref(d), _addr(out), _addr(lse), _addr(ws), _raw_stream()), "cross_attention_fwd")
+        if grad:
+            ctx.save_for_backward(q, k, v, key_mask, kv_lens, out, lse)
+            ctx.scale = scale
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        _once("cross_attention")
+        q, k, v, key_mask, kv_lens, out, lse = ctx.saved_tensors
+        nat.require_device(g, q)
+        lib = nat.lib()
+        d = CrossAttention._desc(q, k, v, key_mask, kv_lens, ctx.scale)
+        g = g.to(q.dtype).contiguous()
+        if g.data_ptr() & 15:
+            g = g.clone()
+        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        states = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        gk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if states else None
+        gv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if states else None
+        ws = torch.empty(lib.mvf_cross_attention_bwd_workspace_bytes(C.byref(d)), dtype=torch.uint8, device=q.device)
+        nat.check(lib.mvf_cross_attention_bwd(C.byref(d), _addr(out), _addr(lse), _addr(g), _addr(gq), _addr(gk), _addr(gv),
+                                              _addr(ws), _raw_stream()), "cross_attention_bwd")
+        need = ctx.needs_input_grad
+        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None
+
+
+def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
+    """Attention of the queries ``q [B, Lq, Hq, D]`` to the states ``k, v [B, Lk, Hk, D]`` of another length -> ``[B, Lq, Hq, D]``.
+
+    ``Hq`` is a multiple of ``Hk``: query head h reads head ``h // (Hq // Hk)`` of the states.  float32 or bfloat16, at most 128
+    channels per head, any strides (channels adjacent; otherwise copied).  ``scale`` (> 0, default ``1 / sqrt(D)``) multiplies
+    the scores.  ``kv_lens`` (integers ``[B]`` on the device): states 0 .. kv_lens[b] - 1 of sequence b count.  ``key_mask`` (bool or
+    uint8 ``[B, Lk]``): the states that count, together with the lengths.  A state that does not count contributes nothing,
+    whatever its memory holds, and gets zero gradients; a query that no state counts for gets zeros.  Differentiable once in
+    q, k and v; both directions are bit-reproducible.  One query per sequence is the same call (the states are split over the chip)."""
+    what = "cross_attention"
+    q = _token_heads(what, "q", q)
+    k, v = _token_heads(what, "k", k, q.dtype), _token_heads(what, "v", v, q.dtype)
+    if k.shape != v.shape:
+        raise RuntimeError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    B, _, Hq, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D or Hq % k.shape[2]:
+        raise RuntimeError(f"{what}: states {tuple(k.shape)} do not fit queries {tuple(q.shape)} (same batch and channels, query "
+                           "heads a multiple of the states' heads)")
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e38:
+        raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, k.shape[1]):
+            raise RuntimeError(f"{what}: key_mask must be bool or uint8 {(B, k.shape[1])}, got {key_mask.dtype} {tuple(key_mask.shape)}")
+    if kv_lens is not None:
+        if kv_lens.dtype not in (torch.int32, torch.int64) or tuple(kv_lens.shape) != (B,):
+            raise RuntimeError(f"{what}: kv_lens must be int32 or int64 {(B,)}, got {kv_lens.dtype} {tuple(kv_lens.shape)}")
+    nat.require_device(q, k, v, key_mask, kv_lens)
+    if kv_lens is not None:
+        kv_lens = kv_lens.clamp(0, k.shape[1]).int() if kv_lens.dtype != torch.int32 else kv_lens
+        kv_lens = kv_lens.contiguous()
+    return CrossAttention.apply(q, k, v, key_mask, kv_lens, scale)
+
+
+@functools.lru_cache(maxsize=64)
+def _turn_fractions(ra, base):
+    """Turns per unit of position of the ra / 2 frequencies, as 64-bit fractions of a turn (a host array; kept alive by the cache)."""
+    f = [int(round(base ** (-2.0 * j / ra) / (2.0 * math.pi) * 2.0 ** 64)) % 2 ** 64 for j in range(ra // 2)]
+    return (C.c_uint64 * max(1, len(f)))(*f)
+
+
+class QkNormRope(torch.autograd.Function):
+    """Norm of every query / key head and rotation by position in one pass (csrc/mvf_qknorm.hip).  No counterpart in the reference."""
+
+    @staticmethod
+    def _desc(q, k, wq, wk, pq, pk, rot, axes, base, eps, interleaved):
+        B, Lq, Hq, D = q.shape
+        d = nat.QkNormDesc(q=_addr(q), k=_addr(k), q_weight=_addr(wq), k_weight=_addr(wk), q_pos=_addr(pq), k_pos=_addr(pk),
+                           freq=C.addressof(_turn_fractions(rot // axes, base)), B=B, Lq=Lq, Lk=0 if k is None else k.shape[1],
+                           Hq=Hq, Hk=1 if k is None else k.shape[2], D=D, dtype=_ATTN_TYPES[q.dtype], axes=axes, rot=rot,
+                           interleaved=interleaved, eps=eps)
+        d.q_stride[:] = q.stride()[:3]
+        if k is not None:
+            d.k_stride[:] = k.stride()[:3]
+        p = pq if pq is not None else pk
+        d.pos64 = p is not None and p.dtype == torch.int64
+        if pq is not None and pq.dim() == 3:
+            d.q_pos_stride = pq.stride(0)
+        if pk is not None and pk.dim() == 3:
+            d.k_pos_stride = pk.stride(0)
+        return d
+
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pq, pk, cfg):
+        d = QkNormRope._desc(q, k, wq, wk, pq, pk, *cfg)
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        nat.check(nat.lib().mvf_qk_norm_rope_fwd(C.byref(d), _addr(yq), _addr(yk), _raw_stream()), "qk_norm_rope_fwd")
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(q, k, wq, wk, pq, pk)
+            ctx.cfg = cfg
+        return yq if k is None else (yq, yk)
+
+    @staticmethod
+    def backward(ctx, gyq, gyk=None):
+        _once("qk_norm_rope")
+        q, k, wq, wk, pq, pk = ctx.saved_tensors
+        nat.require_device(gyq, q, gyk)
+        d = QkNormRope._desc(q, k, wq, wk, pq, pk, *ctx.cfg)
+        lib, need = nat.lib(), ctx.needs_input_grad
+
+        def grad_in(g, x):
+            g = g.to(x.dtype).contiguous()
+            return g.clone() if g.data_ptr() & 15 else g
+        gyq = grad_in(gyq, q)
+        gyk = None if k is None else grad_in(gyk, k)
+        gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        gk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        gwq = torch.empty_like(wq) if need[2] else None
+        gwk = torch.empty_like(wk) if need[3] else None
+        n = lib.mvf_qk_norm_rope_bwd_workspace_floats(C.byref(d)) if need[2] or need[3] else 0
+        ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+        if (need[2] or need[3]) and ws is None:                       # no rows at all
+            gwq, gwk = (None if w is None else w.zero_() for w in (gwq, gwk))
+        else:
+            nat.check(lib.mvf_qk_norm_rope_bwd(C.byref(d), _addr(gyq), _addr(gyk), _addr(gq), _addr(gk), _addr(gwq), _addr(gwk),
+                                               _addr(ws), _raw_stream()), "qk_norm_rope_bwd")
+        return gq if need[0] else None, gk if need[1] else None, gwq, gwk, None, None, None
+
+
+def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, q_pos=None, k_pos=None, *, rot_dim=None, base=10000.0, eps=1e-6,
+                 interleaved=False):
+    """RMS norm of every query and key head, ``x * rsqrt(mean(x^2) + eps) * weight``, and rotation by position, in one pass.
+
+    ``q [B, Lq, Hq, D]``, ``k [B, Lk, Hk, D]`` or None (queries alone: the states of an encoder are normed and rotated once); float32
+    or bfloat16, D <= 128, any strides (channels adjacent; otherwise copied).  Returns ``(q', k')`` or ``q'``, contiguous.
+    ``q_weight``, ``k_weight``: ``[D]`` in float32 or the type of q, or None.  ``q_pos``, ``k_pos``: int32 or int64 ``[L, axes]`` or
+    ``[B, L, axes]`` (``[L]``: one axis), or None for no rotation of that side; up to three axes -- an index; row and column; frame, row
+    and column.  The first ``rot_dim`` channels (default: as many as ``2 * axes`` divides) are ``axes`` equal blocks, one per
+    coordinate; pair j of a block of n channels turns by ``pos * base^(-2 j / n)``; pairs are (j, j + n/2) of the block, or
+    (2j, 2j + 1) if ``interleaved``.  Positions may be any integers, also negative ones: angles do not lose precision far out.
+    Differentiable once in q, k and the weights; both directions are bit-reproducible."""
+    what = "qk_norm_rope"
+    q = _token_heads(what, "q", q)
+    k = None if k is None else _token_heads(what, "k", k, q.dtype)
+    B, _, _, D = q.shape
+    if k is not None and (k.shape[0] != B or k.shape[3] != D):
+        raise RuntimeError(f"{what}: k {tuple(k.shape)} does not fit q {tuple(q.shape)} (same batch and channels)")
+    if k is None and (k_weight is not None or k_pos is not None):
+        raise RuntimeError(f"{what}: k_weight / k_pos without k")
+    axes, pos = None, []
+    for name, p, x in (("q_pos", q_pos, q), ("k_pos", k_pos, k)):
+        if p is not None:
+            if p.dtype not in (torch.int32, torch.int64):
+                raise RuntimeError(f"{what}: {name} must be int32 or int64, got {p.dtype}")
+            p = p[:, None] if p.dim() == 1 else p
+            if p.dim() not in (2, 3) or p.shape[-2] != x.shape[1] or (p.dim() == 3 and p.shape[0] != B) or not 1 <= p.shape[-1] <= 3:
+                raise RuntimeError(f"{what}: {name} must be [{x.shape[1]}, axes] or [{B}, {x.shape[1]}, axes] with 1..3 axes, got "
+                                   f"{tuple(p.shape)}")
+            if axes not in (None, p.shape[-1]):
+                raise RuntimeError(f"{what}: q_pos and k_pos have different numbers of axes")
+            axes = p.shape[-1]
+        pos.append(p)
+    axes = axes or 1
+    rot = D // (2 * axes) * (2 * axes) if rot_dim is None else int(rot_dim)
+    if rot < 0 or rot > D or rot % (2 * axes):
+        raise RuntimeError(f"{what}: rot_dim {rot} must be a multiple of {2 * axes} (two per axis) of at most {D} channels")
+    base, eps = float(base), float(eps)
+    if not 0.0 < base < math.inf or not 0.0 <= eps < math.inf:
+        raise RuntimeError(f"{what}: base must be positive and eps not negative, got {base} and {eps}")
+    w = []
+    for name, x in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if x is not None and (x.dtype not in (torch.float32, q.dtype) or tuple(x.shape) != (D,)):
+            raise RuntimeError(f"{what}: {name} must be [{D}] in float32 or {q.dtype}, got {x.dtype} {tuple(x.shape)}")
+        w.append(x)
+    nat.require_device(q, k, *w, *pos)
+    w = [None if x is None else x.float().contiguous() for x in w]
+    pos = [None if p is None else p.contiguous() for p in pos]
+    if pos[0] is not None and pos[1] is not None and pos[0].dtype != pos[1].dtype:
+        pos = [p.long() for p in pos]
+    return QkNormRope.apply(q, k, w[0], w[1], pos[0], pos[1], (rot, axes, base, eps, bool(interleaved)))
