@@ -101,35 +101,77 @@ MVF_DEV f32x16 mma(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
-// channels d0 .. d0 + 7 of a row of D channels (zeros behind D); `wide`: rows are 16-byte aligned and D a multiple of 8
-MVF_DEV void load8(const float *row, int d0, int D, bool wide, float (&x)[8])
-{
-    if (wide && d0 < D) {
-        const f32x4 a = *(const f32x4 *)(row + d0), b = *(const f32x4 *)(row + d0 + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
-        return;
+// eight channels of a row as loaded
+template <int NP>
+struct Raw;
+template <>
+struct Raw<1> {
+    bf16x8 x;
+    MVF_DEV void zero() { x = bf16x8{}; }
+    MVF_DEV Frag<1> frag() const { return Frag<1>{{x}}; }
+};
+template <>
+struct Raw<3> {
+    f32x4 a, b;
+    MVF_DEV void zero() { a = b = f32x4{}; }
+    MVF_DEV Frag<3> frag() const
+    {
+        const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        return split8<3>(x);
     }
+};
+// channels d0 .. d0 + 7 of a row of D channels (zeros behind D, or if the row is not `live`); `wide`: rows are 16-byte aligned
+// and D is a multiple of 8
+MVF_DEV Raw<1> load8(const __bf16 *row, int d0, int D, bool wide, bool live)
+{
+    Raw<1> r;
+    r.zero();
+    if (!live) return r;
+    if (wide) {
+        if (d0 < D) r.x = *(const bf16x8 *)(row + d0);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = d0 + e < D ? row[d0 + e] : 0.0f;
+        for (int e = 0; e < 8; ++e)
+            if (d0 + e < D) r.x[e] = row[d0 + e];
+    }
+    return r;
+}
+MVF_DEV Raw<3> load8(const float *row, int d0, int D, bool wide, bool live)
+{
+    Raw<3> r;
+    r.zero();
+    if (!live) return r;
+    if (wide) {
+        if (d0 < D) {
+            r.a = *(const f32x4 *)(row + d0);
+            r.b = *(const f32x4 *)(row + d0 + 4);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (d0 + e < D) r.a[e] = row[d0 + e];
+            if (d0 + 4 + e < D) r.b[e] = row[d0 + 4 + e];
+        }
+    }
+    return r;
+}
+// acc + the dot product of two rows' channels
+MVF_DEV float dot8(const Raw<1> &x, const Raw<1> &y, float acc)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf((float)x.x[e], (float)y.x[e], acc);
+    return acc;
+}
+MVF_DEV float dot8(const Raw<3> &x, const Raw<3> &y, float acc)
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc = fmaf(x.b[e], y.b[e], fmaf(x.a[e], y.a[e], acc));
+    return acc;
 }
 template <int NP>
 MVF_DEV Frag<NP> load_frag(const typename Elem<NP>::T *row, int d0, int D, bool wide, bool live)
 {
-    Frag<NP> f;
-    if constexpr (NP == 1) {
-        if (live && wide && d0 < D) {
-            f.p[0] = *(const bf16x8 *)(row + d0);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f.p[0][e] = (live && d0 + e < D) ? row[d0 + e] : (__bf16)0.0f;
-        }
-        return f;
-    } else {
-        float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (live) load8(row, d0, D, wide, x);
-        return split8<NP>(x);
-    }
+    return load8(row, d0, D, wide, live).frag();
 }
 
 // ------------------------------------------------------------------------------------------------- LDS tiles
@@ -219,20 +261,61 @@ MVF_DEV uint64_t live_states(const AttnArgs &a, int b, int j0, int n, int lane)
     return __ballot(ok);
 }
 
-// tile <- rows j0 .. of the states (or query rows) through `row_ptr(row)`; rows that do not count become zeros
-template <int NP, int ROWS, int DP, typename F>
-MVF_DEV void stage(Tile<NP, ROWS, DP> &t, const AttnArgs &a, F row_ptr)
-{
-    constexpr int CPR = DP / 8;
+// This lane's chunks of a tile in flight: fetch() starts the loads of the rows `row_ptr(row)` (nullptr: zeros), commit() puts
+// them into the tile.  The loads of a tile are issued before the products of the one before it.
+template <int NP, int ROWS, int DP>
+struct Flight {
+    static constexpr int CPR = DP / 8, CHUNKS = ROWS * CPR, N = (CHUNKS + NT - 1) / NT;
+    Raw<NP> r[N];
+    template <typename F>
+    MVF_DEV void fetch(const AttnArgs &a, bool wide, F row_ptr)
+    {
 #pragma unroll
-    for (int c0 = 0; c0 < Tile<NP, ROWS, DP>::CHUNKS; c0 += NT) {
-        const int c = c0 + threadIdx.x;
-        if ((Tile<NP, ROWS, DP>::CHUNKS % NT) && c >= Tile<NP, ROWS, DP>::CHUNKS) break;
-        const int row = c / CPR, ch = c - row * CPR;
-        const typename Elem<NP>::T *p = row_ptr(row);
-        t.put(row, ch, load_frag<NP>(p, ch * 8, a.D, a.wide, p != nullptr));
+        for (int i = 0; i < N; ++i) {
+            const int c = i * NT + threadIdx.x, row = c / CPR, ch = c - row * CPR;
+            const bool in = CHUNKS % NT == 0 || c < CHUNKS;
+            const typename Elem<NP>::T *p = in ? row_ptr(row) : nullptr;
+            r[i] = load8(p, ch * 8, a.D, wide, p != nullptr);
+        }
     }
-}
+    MVF_DEV void commit(Tile<NP, ROWS, DP> &t) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = i * NT + threadIdx.x, row = c / CPR, ch = c - row * CPR;
+            if (CHUNKS % NT == 0 || c < CHUNKS) t.put(row, ch, r[i].frag());
+        }
+    }
+};
+
+// The tiles of states a workgroup walks: [j, end) in steps of BK, those without a state that counts left out.  The same in
+// every lane of the workgroup.
+template <int BK>
+struct Walk {
+    int j, end, n, b, lane;
+    uint64_t bits;
+    static constexpr uint64_t kFull = BK == 64 ? ~0ull : (1ull << (BK & 63)) - 1;
+    MVF_DEV Walk(const AttnArgs &a, int b_, int part, int lane_) : b(b_), lane(lane_), bits(0)
+    {
+        n = states_of(a, b);
+        j = part * a.per * BK;
+        end = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * BK);
+        settle(a);
+    }
+    MVF_DEV bool live() const { return j < end; }
+    MVF_DEV void next(const AttnArgs &a)
+    {
+        j += BK;
+        settle(a);
+    }
+    MVF_DEV void settle(const AttnArgs &a)
+    {
+        for (; j < end; j += BK) {
+            bits = live_states(a, b, j, n, lane) & kFull;
+            if (bits) return;
+        }
+    }
+};
 
 MVF_DEV float other_half_max(float x)
 {
@@ -293,13 +376,35 @@ MVF_DEV void store_cols(T *row, const f32x16 (&acc)[DT], float f, int D, bool wi
                    acc[t][4 * i + 3] * f);
 }
 
+// NP == 3: the products of a tile are summed on their own and then added to the running sum, so that its roundings are one per
+// tile and not one per matrix instruction (3,840 states: error 5e-6 -> 1e-6 of the result)
+template <int NP, int DT, int ROWS, int DP>
+MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, const f32x16 &x, int lane)
+{
+    const Frag<NP> x0 = acc_frag<NP>(x, 0), x1 = acc_frag<NP>(x, 1);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        if constexpr (NP == 1) {
+            acc[d] = mma(t.cols(32 * d, r0, lane), x0, acc[d]);
+            acc[d] = mma(t.cols(32 * d, r0 + 16, lane), x1, acc[d]);
+        } else {
+            f32x16 y = {};
+            y = mma(t.cols(32 * d, r0, lane), x0, y);
+            y = mma(t.cols(32 * d, r0 + 16, lane), x1, y);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] += y[i];
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------- forward
-// grid: (batch x key head) major, then the part of the states, then the row tile (128 rows)
-template <int NP, int DP, int BK>
+// grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x QT x 32 rows)
+template <int NP, int DP, int BK, int QT>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
     constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
+    constexpr float kSlack = 8.0f;            // the reference of the exponentials follows the maximum once it is 2^8 behind
     __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tk;
     __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
@@ -307,124 +412,105 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int r = tile * 128 + wave * 32 + col;
-    const bool live = r < a.R;
-    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
-    Frag<NP> qf[KS];
-#pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, a.wide, live);
-    f32x16 o[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    const int n = states_of(a, b);
+    const int rw = (tile * 4 + wave) * QT * 32 + col;             // this lane's first row
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
-    const int j1 = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * BK);
-    for (int j0 = part * a.per * BK; j0 < j1; j0 += BK) {
-        uint64_t bits = live_states(a, b, j0, n, lane);
-        if (BK < 64) bits &= (1ull << (BK & 63)) - 1;
-        if (bits == 0) continue;
+    const bool wide = a.wide;
+    Walk<BK> w(a, b, part, lane);
+    Flight<NP, BK, DP> fk, fv;
+    auto fetch = [&] {
+        fk.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? kb + (int64_t)(w.j + row) * a.ks[1] : (const T *)nullptr; });
+        fv.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? vb + (int64_t)(w.j + row) * a.vs[1] : (const T *)nullptr; });
+    };
+    if (w.live()) fetch();
+    Frag<NP> qf[QT][KS];
+    f32x16 o[QT][DT];
+    float m[QT], sub[QT], l[QT];              // reference and sum of the exponentials; sub: the reference, 0 while there is none
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = rw + 32 * q;
+        const T *row = (const T *)a.q + (r < a.R ? row_off(a.qs, b, r, hk, a.G) : 0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[q][s] = load_frag<NP>(row, 16 * s + 8 * h, a.D, wide, r < a.R);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[q][t] = f32x16{};
+        m[q] = -INFINITY;
+        sub[q] = l[q] = 0.0f;
+    }
+    while (w.live()) {
+        const uint64_t bits = w.bits;
         __syncthreads();
-        stage(tk, a, [&](int row) { return (bits >> row) & 1 ? kb + (int64_t)(j0 + row) * a.ks[1] : (const T *)nullptr; });
-        stage(tv, a, [&](int row) { return (bits >> row) & 1 ? vb + (int64_t)(j0 + row) * a.vs[1] : (const T *)nullptr; });
+        fk.commit(tk);
+        fv.commit(tv);
         __syncthreads();
-        f32x16 s[KT];
+        w.next(a);
+        if (w.live()) fetch();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
+            f32x16 s[QT];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+            for (int q = 0; q < QT; ++q) s[q] = f32x16{};
 #pragma unroll
-            for (int x = 0; x < KS; ++x) s[t] = mma(tk.rows(32 * t, 16 * x, lane), qf[x], s[t]);
-        }
-        const uint64_t full = BK < 64 ? (1ull << (BK & 63)) - 1 : ~0ull;
-        if (bits != full) {
+            for (int x = 0; x < KS; ++x) {
+                const Frag<NP> kf = tk.rows(32 * t, 16 * x, lane);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const uint32_t w = (uint32_t)(bits >> (32 * t)) >> (4 * h);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((w >> acc_row(i, 0)) & 1)) s[t][i] = -INFINITY;
+                for (int q = 0; q < QT; ++q) s[q] = mma(kf, qf[q][x], s[q]);
             }
-        }
-        float mx = s[0][0];
+            if (bits != Walk<BK>::kFull) {
+                const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+                for (int q = 0; q < QT; ++q)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = fmaxf(m, other_half_max(mx));
-        const float mc = (mx == -INFINITY ? 0.0f : mx) * a.c;
-        const float f = __builtin_amdgcn_exp2f(fmaf(m, a.c, -mc));
-        m = mx;
-        l *= f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] *= f;
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.c, -mc));
-                l += p;
-                s[t][i] = p;
+                    for (int i = 0; i < 16; ++i)
+                        if (!((ok >> acc_row(i, 0)) & 1)) s[q][i] = -INFINITY;
             }
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+            for (int q = 0; q < QT; ++q) {
+                float mx = s[q][0];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const Frag<NP> p = acc_frag<NP>(s[t], x);
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[q][i]);
+                mx = other_half_max(mx) * a.c;
+                if (__any(mx > m[q] + kSlack)) {
+                    mx = fmaxf(mx, m[q]);
+                    const float f = __builtin_amdgcn_exp2f(m[q] - (mx == -INFINITY ? 0.0f : mx));
+                    m[q] = mx;
+                    sub[q] = mx == -INFINITY ? 0.0f : mx;
+                    l[q] *= f;
 #pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] = mma(tv.cols(32 * d, 32 * t + 16 * x, lane), p, o[d]);
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[q][d][i] *= f;
+                }
+                float lt = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[q][i] = __builtin_amdgcn_exp2f(fmaf(s[q][i], a.c, -sub[q]));
+                    lt += s[q][i];
+                }
+                l[q] += lt;
             }
-    }
-    l = other_half_sum(l);
-    if (!live) return;
-    if (a.splits > 1) {                                          // this part's maximum, sum and unscaled output
-        const int64_t w = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
-        store_cols<DT>(a.part + w * a.D, o, 1.0f, a.D, (a.D & 3) == 0, h);
-        if (h == 0) {
-            a.part2[2 * w] = m * a.c;
-            a.part2[2 * w + 1] = l;
-        }
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, (a.D & 7) == 0, h);
-    if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l));
-}
-
-// joins the parts of a row: o = sum_p o_p 2^(m_p - m) / sum_p l_p 2^(m_p - m).  One lane per four channels.
-template <typename T>
-__global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a)
-{
-    const int per = (a.D + 3) / 4;
-    const int64_t idx = (int64_t)blockIdx.x * NT + threadIdx.x, rows = (int64_t)a.B * a.Hk * a.R;
-    const int64_t w = idx / per;
-    if (w >= rows) return;
-    const int d = (int)(idx - w * per) * 4;
-    float m = -INFINITY;
-    for (int p = 0; p < a.splits; ++p) {
-        const int64_t y = p * rows + w;
-        if (a.part2[2 * y + 1] != 0.0f) m = fmaxf(m, a.part2[2 * y]);
-    }
-    float l = 0.0f, o[4] = {0, 0, 0, 0};
-    for (int p = 0; p < a.splits; ++p) {
-        const int64_t y = p * rows + w;
-        const float lp = a.part2[2 * y + 1];
-        if (lp == 0.0f) continue;                                // nothing counted in this part
-        const float f = __builtin_amdgcn_exp2f(a.part2[2 * y] - m);
-        l = fmaf(lp, f, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (d + i < a.D) o[i] = fmaf(a.part[y * a.D + d + i], f, o[i]);
+            for (int q = 0; q < QT; ++q) accumulate<NP>(o[q], tv, 32 * t, s[q], lane);
+        }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int bh = (int)(w / a.R), r = (int)(w - (int64_t)bh * a.R), b = bh / a.Hk, hk = bh - b * a.Hk;
-    store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 7) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    if (a.lse && d == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = rw + 32 * q;
+        const float lq = other_half_sum(l[q]);
+        if (r >= a.R) continue;
+        if (a.splits > 1) {                                      // this part's reference, sum and unscaled output
+            const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+            store_cols<DT>(a.part + y * a.D, o[q], 1.0f, a.D, (a.D & 3) == 0, h);
+            if (h == 0) {
+                a.part2[2 * y] = m[q];
+                a.part2[2 * y + 1] = lq;
+            }
+            continue;
+        }
+        const float inv = lq == 0.0f ? 0.0f : 1.0f / lq;
+        store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o[q], inv, a.D, (a.D & 7) == 0, h);
+        if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = lq == 0.0f ? INFINITY : m[q] + __builtin_amdgcn_logf(lq);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------- backward
@@ -434,7 +520,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a)
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
 // grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
-template <int NP, int DP, int BK>
+template <int NP, int DP, int BK, int QT>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
@@ -446,82 +532,97 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int r = tile * 128 + wave * 32 + col;
-    const bool live = r < a.R;
-    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
-    const int64_t dense = live ? dense_row(b, r, hk, a) : 0;
-    const bool dwide = (a.D & 7) == 0;
-    Frag<NP> qf[KS], gf[KS];
-    float delta = 0.0f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, a.wide, live);
-        gf[s] = load_frag<NP>((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
-        const T *orow = (const T *)a.o + dense, *grow = (const T *)a.go + dense;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = 16 * s + 8 * h + e;
-            if (live && d < a.D) delta = fmaf((float)grow[d], (float)orow[d], delta);
-        }
-    }
-    delta = other_half_sum(delta);
-    const float lse = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
-    if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta;
-    f32x16 dq[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dq[t][i] = 0.0f;
-    const int n = states_of(a, b);
+    const int rw = (tile * 4 + wave) * QT * 32 + col;
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
-    const int j1 = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * BK);
-    for (int j0 = part * a.per * BK; j0 < j1; j0 += BK) {
-        uint64_t bits = live_states(a, b, j0, n, lane);
-        if (BK < 64) bits &= (1ull << (BK & 63)) - 1;
-        if (bits == 0) continue;
+    const bool wide = a.wide, dwide = (a.D & 7) == 0;
+    Walk<BK> w(a, b, part, lane);
+    Flight<NP, BK, DP> fk, fv;
+    auto fetch = [&] {
+        fk.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? kb + (int64_t)(w.j + row) * a.ks[1] : (const T *)nullptr; });
+        fv.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? vb + (int64_t)(w.j + row) * a.vs[1] : (const T *)nullptr; });
+    };
+    if (w.live()) fetch();
+    Frag<NP> qf[QT][KS], gf[QT][KS];
+    f32x16 dq[QT][DT];
+    float delta[QT], lse[QT];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = rw + 32 * q;
+        const bool live = r < a.R;
+        const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
+        const int64_t dense = live ? dense_row(b, r, hk, a) : 0;
+        float de = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            qf[q][s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, wide, live);
+            const Raw<NP> g = load8((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
+            de = dot8(g, load8((const T *)a.o + dense, 16 * s + 8 * h, a.D, dwide, live), de);
+            gf[q][s] = g.frag();
+        }
+        delta[q] = other_half_sum(de);
+        lse[q] = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
+        if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta[q];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) dq[q][t] = f32x16{};
+    }
+    while (w.live()) {
+        const uint64_t bits = w.bits;
         __syncthreads();
-        stage(tk, a, [&](int row) { return (bits >> row) & 1 ? kb + (int64_t)(j0 + row) * a.ks[1] : (const T *)nullptr; });
-        stage(tv, a, [&](int row) { return (bits >> row) & 1 ? vb + (int64_t)(j0 + row) * a.vs[1] : (const T *)nullptr; });
+        fk.commit(tk);
+        fv.commit(tv);
         __syncthreads();
+        w.next(a);
+        if (w.live()) fetch();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            f32x16 s, dp;
+            f32x16 s[QT], dp[QT];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+            for (int q = 0; q < QT; ++q) s[q] = dp[q] = f32x16{};
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
-                s = mma(tk.rows(32 * t, 16 * x, lane), qf[x], s);
-                dp = mma(tv.rows(32 * t, 16 * x, lane), gf[x], dp);
+                const Frag<NP> kf = tk.rows(32 * t, 16 * x, lane), vf = tv.rows(32 * t, 16 * x, lane);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) {
+                    s[q] = mma(kf, qf[q][x], s[q]);
+                    dp[q] = mma(vf, gf[q][x], dp[q]);
+                }
             }
             // a state that does not count: its row of the tile is zero, so whatever dS holds for it adds nothing to dq --
             // but exp2(-lse) may be infinite there, so it is cleared
-            const uint32_t w = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+            const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+            if (bits != Walk<BK>::kFull) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = (w >> acc_row(i, 0)) & 1 ? __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) : 0.0f;
-                s[i] = p * (dp[i] - delta);
+                for (int q = 0; q < QT; ++q)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((ok >> acc_row(i, 0)) & 1)) s[q][i] = -INFINITY;
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const Frag<NP> ds = acc_frag<NP>(s, x);
+            for (int q = 0; q < QT; ++q)
 #pragma unroll
-                for (int d = 0; d < DT; ++d) dq[d] = mma(tk.cols(32 * d, 32 * t + 16 * x, lane), ds, dq[d]);
-            }
+                for (int i = 0; i < 16; ++i)
+                    s[q][i] = __builtin_amdgcn_exp2f(fmaf(s[q][i], a.c, -lse[q])) * (dp[q][i] - delta[q]);
+#pragma unroll
+            for (int q = 0; q < QT; ++q) accumulate<NP>(dq[q], tk, 32 * t, s[q], lane);
         }
     }
-    if (!live) return;
-    if (a.splits > 1) {
-        const int64_t w = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
-        store_cols<DT>(a.part + w * a.D, dq, a.scale, a.D, (a.D & 3) == 0, h);
-        return;
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+        const int r = rw + 32 * q;
+        if (r >= a.R) continue;
+        if (a.splits > 1) {
+            const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+            store_cols<DT>(a.part + y * a.D, dq[q], a.scale, a.D, (a.D & 3) == 0, h);
+            continue;
+        }
+        store_cols<DT>((T *)a.dq + dense_row(b, r, hk, a), dq[q], a.scale, a.D, dwide, h);
     }
-    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, dwide, h);
 }
 
-// grid: (batch x key head) major, then the part of the rows, then the state tile (128 states, 32 per wave).  Row tiles of q and
+// grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x KT x 32 states).  Row tiles of q and
 // do are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS
-template <int NP, int DP, int BQ>
+template <int NP, int DP, int BQ, int KT>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
@@ -534,123 +635,189 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int j = tile * 128 + wave * 32 + col;
-    const int n = states_of(a, b);
-    const bool mine = j < a.Lk;
-    bool live = j < n;
-    if (live && a.mask) live = a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0;
-    const T *krow = (const T *)a.k + (live ? (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)hk * a.ks[2] : 0);
-    const T *vrow = (const T *)a.v + (live ? (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)hk * a.vs[2] : 0);
-    Frag<NP> kf[KS], vf[KS];
+    const int jw = (tile * 4 + wave) * KT * 32 + col, n = states_of(a, b);
+    const bool wide = a.wide, dwide = (a.D & 7) == 0;
+    Frag<NP> kf[KT][KS], vf[KT][KS];
+    f32x16 dk[KT][DT], dv[KT][DT];
+    bool live[KT];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        kf[s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, a.wide, live);
-        vf[s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, a.wide, live);
+    for (int t = 0; t < KT; ++t) {
+        const int j = jw + 32 * t;
+        live[t] = j < n && (!a.mask || a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0);
+        const T *krow = (const T *)a.k + (live[t] ? (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)hk * a.ks[2] : 0);
+        const T *vrow = (const T *)a.v + (live[t] ? (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)hk * a.vs[2] : 0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            kf[t][s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, wide, live[t]);
+            vf[t][s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, wide, live[t]);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x16{};
     }
-    f32x16 dk[DT], dv[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.0f;
-    const int r1 = (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ);
-    const bool any = tile * 128 < n;                              // (the same in every lane of the workgroup)
-    for (int r0 = part * a.per * BQ; any && r0 < r1; r0 += BQ) {
-        __syncthreads();
-        stage(tq, a, [&](int row) { return r0 + row < a.R ? (const T *)a.q + row_off(a.qs, b, r0 + row, hk, a.G) : (const T *)nullptr; });
-        stage(tg, a, [&](int row) { return r0 + row < a.R ? (const T *)a.go + dense_row(b, r0 + row, hk, a) : (const T *)nullptr; });
+    const int r1 = tile * 4 * KT * 32 < n ? (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ) : 0;
+    int r0 = part * a.per * BQ;
+    Flight<NP, BQ, DP> fq, fg;
+    float pl = 0.0f, pd = 0.0f;
+    auto fetch = [&] {
+        fq.fetch(a, wide, [&](int row) { return r0 + row < a.R ? (const T *)a.q + row_off(a.qs, b, r0 + row, hk, a.G) : (const T *)nullptr; });
+        fg.fetch(a, dwide, [&](int row) { return r0 + row < a.R ? (const T *)a.go + dense_row(b, r0 + row, hk, a) : (const T *)nullptr; });
         if (threadIdx.x < BQ) {
             const int r = r0 + threadIdx.x;
-            sl[threadIdx.x] = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;      // rows behind the last: P = 0
-            sd[threadIdx.x] = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.0f;
+            pl = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;            // rows behind the last: P = 0
+            pd = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.0f;
+        }
+    };
+    if (r0 < r1) fetch();
+    while (r0 < r1) {
+        __syncthreads();
+        fq.commit(tq);
+        fg.commit(tg);
+        if (threadIdx.x < BQ) {
+            sl[threadIdx.x] = pl;
+            sd[threadIdx.x] = pd;
         }
         __syncthreads();
+        r0 += BQ;
+        if (r0 < r1) fetch();
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            f32x16 s, dp;
+        for (int u = 0; u < QT; ++u) {
+            f32x16 s[KT], dp[KT];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.0f;
+            for (int t = 0; t < KT; ++t) s[t] = dp[t] = f32x16{};
 #pragma unroll
             for (int x = 0; x < KS; ++x) {
-                s = mma(tq.rows(32 * t, 16 * x, lane), kf[x], s);
-                dp = mma(tg.rows(32 * t, 16 * x, lane), vf[x], dp);
+                const Frag<NP> qf = tq.rows(32 * u, 16 * x, lane), gf = tg.rows(32 * u, 16 * x, lane);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    s[t] = mma(qf, kf[t][x], s[t]);
+                    dp[t] = mma(gf, vf[t][x], dp[t]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 ls = *(const f32x4 *)&sl[32 * t + acc_row(4 * i, h)], de = *(const f32x4 *)&sd[32 * t + acc_row(4 * i, h)];
+                const f32x4 ls = *(const f32x4 *)&sl[32 * u + acc_row(4 * i, h)], de = *(const f32x4 *)&sd[32 * u + acc_row(4 * i, h)];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = live ? __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], a.c, -ls[e])) : 0.0f;
-                    s[4 * i + e] = p;
-                    dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
-                }
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // (the column of a state that does not count is dropped at the end)
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][4 * i + e], a.c, -ls[e]));
+                        s[t][4 * i + e] = p;
+                        dp[t][4 * i + e] = p * (dp[t][4 * i + e] - de[e]);
+                    }
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const Frag<NP> p = acc_frag<NP>(s, x), ds = acc_frag<NP>(dp, x);
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    dv[d] = mma(tg.cols(32 * d, 32 * t + 16 * x, lane), p, dv[d]);
-                    dk[d] = mma(tq.cols(32 * d, 32 * t + 16 * x, lane), ds, dk[d]);
-                }
+            for (int t = 0; t < KT; ++t) {
+                accumulate<NP>(dv[t], tg, 32 * u, s[t], lane);
+                accumulate<NP>(dk[t], tq, 32 * u, dp[t], lane);
             }
         }
     }
-    if (!mine) return;
-    if (a.splits > 1) {
-        const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, w = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
-        const bool pw = (a.D & 3) == 0;
-        store_cols<DT>(a.part + w, dk, live ? a.scale : 0.0f, a.D, pw, h);
-        store_cols<DT>(a.part + w + n1, dv, 1.0f, a.D, pw, h);
-        return;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const int j = jw + 32 * t;
+        if (j >= a.Lk) continue;
+        if (!live[t]) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x16{};
+        }
+        if (a.splits > 1) {
+            const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, y = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
+            const bool pw = (a.D & 3) == 0;
+            store_cols<DT>(a.part + y, dk[t], a.scale, a.D, pw, h);
+            store_cols<DT>(a.part + y + n1, dv[t], 1.0f, a.D, pw, h);
+            continue;
+        }
+        const int64_t y = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
+        store_cols<DT>((T *)a.dk + y, dk[t], a.scale, a.D, dwide, h);
+        store_cols<DT>((T *)a.dv + y, dv[t], 1.0f, a.D, dwide, h);
     }
-    const int64_t w = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
-    store_cols<DT>((T *)a.dk + w, dk, a.scale, a.D, (a.D & 7) == 0, h);
-    store_cols<DT>((T *)a.dv + w, dv, 1.0f, a.D, (a.D & 7) == 0, h);
 }
 
-// adds the parts of a gradient, in order.  KV: part[p][2][B * Hk][Lk][D] -> dk, dv [B, Lk, Hk, D]; otherwise part[p][B * Hk][R][D] -> dq
-template <typename T, bool KV>
-__global__ void __launch_bounds__(NT) k_attn_sum(const AttnArgs a)
+// ------------------------------------------------------------------------------------------------- joining parts
+// A wave per row: `per` lanes hold four channels each, 64 / per groups of lanes take every (64 / per)-th part, and a butterfly
+// adds the groups: one fixed order.  (A lane that walked 60 parts by itself took 56 us of a single-token call.)
+//   MODE 0: o = sum_p o_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), and the row's lse
+//   MODE 1: dq = sum_p dq_p;  MODE 2: dk and dv, part[p][2][B * Hk][Lk][D]
+template <typename T, int MODE>
+__global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int64_t total)
 {
-    const int per = (a.D + 3) / 4, len = KV ? a.Lk : a.R;
-    const int64_t idx = (int64_t)blockIdx.x * NT + threadIdx.x, rows = (int64_t)a.B * a.Hk * len;
-    int64_t w = idx / per;
-    const int d = (int)(idx - w * per) * 4;
-    const int which = KV && w >= rows;
-    if (which) w -= rows;
-    if (w >= rows) return;
-    float x[4] = {0, 0, 0, 0};
-    for (int p = 0; p < a.splits; ++p) {
-        const float *y = a.part + (((KV ? 2 * p + which : p) * rows) + w) * a.D + d;
+    const int lane = threadIdx.x & 63, c = lane & (per - 1), pg = lane / per, groups = 64 / per, d = 4 * c;
+    const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    if (row >= total) return;
+    const int len = MODE == 2 ? a.Lk : a.R;
+    const int64_t rows = (int64_t)a.B * a.Hk * len;
+    const int which = MODE == 2 && row >= rows;
+    const int64_t w = which ? row - rows : row;
+    float f = 1.0f, l = 0.0f, m = 0.0f;
+    if (MODE == 0) {                                             // (at most 64 parts: one per lane)
+        const bool in = lane < a.splits;
+        const float lp = in ? a.part2[2 * (lane * rows + w) + 1] : 0.0f, mp = in && lp != 0.0f ? a.part2[2 * (lane * rows + w)] : -INFINITY;
+        m = mp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (d + i < a.D) x[i] += y[i];
+        for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+        f = lp == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mp - m);  // parts without a state that counts: weight 0
+        l = lp * f;
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x, 64);
     }
+    float o[4] = {0, 0, 0, 0};
+    const bool quad = (a.D & 3) == 0;
+    const int64_t step = (MODE == 2 ? 2 : 1) * rows * a.D;
+    const float *src = a.part + (which * rows + w) * a.D + d;
+#pragma unroll 4
+    for (int p0 = 0; p0 < a.splits; p0 += groups) {
+        const int p = p0 + pg;
+        const float wt = MODE == 0 ? __shfl(f, p & 63, 64) : 1.0f;
+        if (p < a.splits && d < a.D && wt != 0.0f) {
+            const float *y = src + p * step;
+            if (quad) {
+                const f32x4 v = *(const f32x4 *)y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = fmaf(v[i], wt, o[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d + i < a.D) o[i] = fmaf(y[i], wt, o[i]);
+            }
+        }
+    }
+    for (int x = per; x < 64; x <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+    if (pg) return;
     const int bh = (int)(w / len), r = (int)(w - (int64_t)bh * len), b = bh / a.Hk, hk = bh - b * a.Hk;
-    T *dst = KV ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D : (T *)a.dq + dense_row(b, r, hk, a);
-    store4(dst, d, a.D, (a.D & 7) == 0, x[0], x[1], x[2], x[3]);
+    const float inv = MODE == 0 ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+    T *dst = MODE == 2 ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D
+                       : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
+    store4(dst, d, a.D, (a.D & 7) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (MODE == 0 && a.lse && c == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
 constexpr int kWant = 512;         // workgroups that fill the chip (two per CU)
 
-// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: enough to fill the chip, at least
-// four tiles each, at most 64
+// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: none if those fill the chip, otherwise
+// enough to, with at least four tiles each, at most 64
 void split_of(int64_t blocks, int red, int &splits, int &per)
 {
-    int64_t s = blocks > 0 ? (kWant + blocks - 1) / blocks : 1;
-    s = s > 64 ? 64 : s;
-    const int most = red / 4 > 1 ? red / 4 : 1;
-    if (s > most) s = most;
-    per = s > 0 ? (int)((red + s - 1) / s) : red;
+    int64_t s = blocks > 0 && blocks < kWant * 3 / 4 ? kWant / blocks : 1;
+    if (s > 64) s = 64;
+    if (s > red / 4) s = red / 4;
+    if (s < 1) s = 1;
+    per = (int)((red + s - 1) / s);
     if (per < 1) per = 1;
     splits = red > 0 ? (red + per - 1) / per : 1;
 }
 
+// two 32-row tiles per wave halve the LDS reads per product; they fit the registers of one plane up to 64 channels
+constexpr bool two_tiles(int NP, int DP) { return NP == 1 && DP <= 64; }
+
 struct Plan {
     int NP, DP, BK, BQ;
-    int rtiles, ktiles;                      // 128-row tiles, 128-state tiles
-    int fs, fper, qs, qper, ks, kper;        // forward, dq, dkv
+    int fq, qq, kk;                          // 32-row (32-state) tiles per wave: forward, dq, dkv
+    int ftiles, qtiles, ktiles;              // workgroups along the rows (states)
+    int fs, fper, qs, qper, ks, kper;        // parts of the reduction, and tiles of a part
 };
 Plan plan_of(const mvf_attn_desc &d)
 {
@@ -660,12 +827,15 @@ Plan plan_of(const mvf_attn_desc &d)
     p.BK = p.NP == 1 ? 64 : 32;
     p.BQ = 32;
     const int R = d.Lq * (d.Hq / d.Hk);
-    p.rtiles = (R + 127) / 128;
-    p.ktiles = (d.Lk + 127) / 128;
     const int64_t bh = (int64_t)d.B * d.Hk;
-    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
-    p.qs = p.fs;
-    p.qper = p.fper;
+    p.fq = two_tiles(p.NP, p.DP) && bh * (R / 256) >= kWant ? 2 : 1;
+    p.qq = p.fq;
+    p.kk = two_tiles(p.NP, p.DP) && bh * (d.Lk / 256) >= kWant ? 2 : 1;
+    p.ftiles = (R + 128 * p.fq - 1) / (128 * p.fq);
+    p.qtiles = (R + 128 * p.qq - 1) / (128 * p.qq);
+    p.ktiles = (d.Lk + 128 * p.kk - 1) / (128 * p.kk);
+    split_of(bh * p.ftiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
+    split_of(bh * p.qtiles, (d.Lk + p.BK - 1) / p.BK, p.qs, p.qper);
     split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, p.ks, p.kper);
     return p;
 }
@@ -679,8 +849,6 @@ bool bad_desc(const mvf_attn_desc *d)
     if (R > (1 << 30) || d->Lk > (1 << 30) || bh * ((R + 127) / 128 + (d->Lk + 127) / 128 + 1) * 64 > 0x7fffffffLL) return true;
     return false;
 }
-int64_t elem_blocks(int64_t n) { return (n + NT - 1) / NT; }
-
 AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
 {
     AttnArgs a = {};
@@ -704,19 +872,45 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
 }
 
 template <int NP, int DP>
-void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_fwd(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_attn_fwd<NP, DP, NP == 1 ? 64 : 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    constexpr int BK = NP == 1 ? 64 : 32;
+    if constexpr (two_tiles(NP, DP))
+        if (tiles == 2) {
+            hipLaunchKernelGGL((k_attn_fwd<NP, DP, BK, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((k_attn_fwd<NP, DP, BK, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
-void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_dq(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_attn_dq<NP, DP, NP == 1 ? 64 : 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    constexpr int BK = NP == 1 ? 64 : 32;
+    if constexpr (two_tiles(NP, DP))
+        if (tiles == 2) {
+            hipLaunchKernelGGL((k_attn_dq<NP, DP, BK, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((k_attn_dq<NP, DP, BK, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
-void launch_dkv(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_dkv(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    if constexpr (two_tiles(NP, DP))
+        if (tiles == 2) {
+            hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+            return;
+        }
+    hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+}
+template <int MODE>
+void launch_join(const AttnArgs &a, int NP, int64_t rows, hipStream_t st)
+{
+    int per = 1;
+    while (per * 4 < a.D) per *= 2;
+    const dim3 g((unsigned)((rows + NT / 64 - 1) / (NT / 64)));
+    if (NP == 1) hipLaunchKernelGGL((k_attn_join<__bf16, MODE>), g, dim3(NT), 0, st, a, per, rows);
+    else hipLaunchKernelGGL((k_attn_join<float, MODE>), g, dim3(NT), 0, st, a, per, rows);
 }
 #define MVF_ATTN_PICK(fn, p, ...)                                                                      \
     do {                                                                                               \
@@ -758,17 +952,13 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     const int64_t rows = (int64_t)d->B * d->Hq * d->Lq;
     a.out = out;
     a.lse = lse;
-    a.tiles = p.rtiles; a.splits = p.fs; a.per = p.fper;
+    a.tiles = p.ftiles; a.splits = p.fs; a.per = p.fper;
     a.part = (float *)workspace;
     a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
-    MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
-    if (p.fs > 1) {
-        const int64_t nb = elem_blocks(rows * ((d->D + 3) / 4));
-        if (p.NP == 1) hipLaunchKernelGGL(k_attn_join<__bf16>, dim3((unsigned)nb), dim3(NT), 0, st, a);
-        else hipLaunchKernelGGL(k_attn_join<float>, dim3((unsigned)nb), dim3(NT), 0, st, a);
-    }
+    MVF_ATTN_PICK(launch_fwd, p, a, p.fq, (int64_t)d->B * d->Hk * p.ftiles * p.fs, st);
+    if (p.fs > 1) launch_join<0>(a, p.NP, rows, st);
     return hip_check_launch();
 }
 
@@ -801,22 +991,14 @@ int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_BWD, st, tensor_bytes(*d, 4 * rows + 4 * states));
     if (d->Lq > 0) {
-        a.tiles = p.rtiles; a.splits = p.qs; a.per = p.qper;
-        MVF_ATTN_PICK(launch_dq, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.qs, st);
-        if (p.qs > 1) {
-            const int64_t nb = elem_blocks(rows * ((d->D + 3) / 4));
-            if (p.NP == 1) hipLaunchKernelGGL((k_attn_sum<__bf16, false>), dim3((unsigned)nb), dim3(NT), 0, st, a);
-            else hipLaunchKernelGGL((k_attn_sum<float, false>), dim3((unsigned)nb), dim3(NT), 0, st, a);
-        }
+        a.tiles = p.qtiles; a.splits = p.qs; a.per = p.qper;
+        MVF_ATTN_PICK(launch_dq, p, a, p.qq, (int64_t)d->B * d->Hk * p.qtiles * p.qs, st);
+        if (p.qs > 1) launch_join<1>(a, p.NP, rows, st);
     }
     if (d->Lk > 0 && g_k) {
         a.tiles = p.ktiles; a.splits = p.ks; a.per = p.kper;
-        MVF_ATTN_PICK(launch_dkv, p, a, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
-        if (p.ks > 1) {
-            const int64_t nb = elem_blocks(2 * states * ((d->D + 3) / 4));
-            if (p.NP == 1) hipLaunchKernelGGL((k_attn_sum<__bf16, true>), dim3((unsigned)nb), dim3(NT), 0, st, a);
-            else hipLaunchKernelGGL((k_attn_sum<float, true>), dim3((unsigned)nb), dim3(NT), 0, st, a);
-        }
+        MVF_ATTN_PICK(launch_dkv, p, a, p.kk, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
+        if (p.ks > 1) launch_join<2>(a, p.NP, 2 * states, st);
     }
     return hip_check_launch();
 }
