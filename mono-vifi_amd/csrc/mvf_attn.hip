@@ -35,8 +35,12 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NT = 256;            // four waves
-constexpr int PADE = 8;            // bf16 elements appended to an LDS row: 16-byte row reads of 16 lanes hit 64 different banks
+constexpr int PADE = 8;            // bf16 elements appended to an LDS row: rows 16 bytes apart modulo 128
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Staged tiles: two buffers (one barrier per tile) for one plane, one buffer (two barriers) for three, whose tiles would halve
+// the number of resident workgroups (1,920 x 3,840 x 32 fp32 forward: 264 against 285 us)
+constexpr int buffers(int NP) { return NP == 1 ? 2 : 1; }
 
 #define LDS_PTR(T) __attribute__((address_space(3))) T *
 
@@ -61,8 +65,8 @@ MVF_DEV short top16(float x) { return (short)(__float_as_uint(x) >> 16); }
 
 // eight fp32 values -> NP planes of bf16.  One plane rounds to nearest even (half a step, 2^-8 of the value); three planes
 // cut, so that every remainder is exact.  (An infinity stays in plane 0 and leaves no remainder: what it multiplies becomes
-// infinite, or NaN where the other factor has an empty plane.)
-template <int NP>
+// infinite, or NaN where the other factor has an empty plane.  Probabilities and dS need no such care: INF false.)
+template <int NP, bool INF = true>
 MVF_DEV Frag<NP> split8(const float (&x)[8])
 {
     Frag<NP> f;
@@ -74,7 +78,7 @@ MVF_DEV Frag<NP> split8(const float (&x)[8])
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float hi = trunc_bf16(x[e]);
-            const float r1 = __builtin_isinf(hi) ? 0.0f : x[e] - hi;
+            const float r1 = INF && __builtin_isinf(hi) ? 0.0f : x[e] - hi;
             const float mid = trunc_bf16(r1);
             a[e] = top16(hi);
             b[e] = top16(mid);
@@ -108,12 +112,18 @@ template <>
 struct Raw<1> {
     bf16x8 x;
     MVF_DEV void zero() { x = bf16x8{}; }
+    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at) { x = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0)); }
     MVF_DEV Frag<1> frag() const { return Frag<1>{{x}}; }
 };
 template <>
 struct Raw<3> {
     f32x4 a, b;
     MVF_DEV void zero() { a = b = f32x4{}; }
+    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at)
+    {
+        a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
+        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 16, 0, 0));
+    }
     MVF_DEV Frag<3> frag() const
     {
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -178,7 +188,7 @@ MVF_DEV Frag<NP> load_frag(const typename Elem<NP>::T *row, int d0, int D, bool 
 // a tile of ROWS x DP values: NP planes of [ROWS][DP + PADE] bf16
 template <int NP, int ROWS, int DP>
 struct Tile {
-    static constexpr int LD = DP + PADE, PLANE = ROWS * LD, CHUNKS = ROWS * (DP / 8);
+    static constexpr int LD = DP + PADE, PLANE = ROWS * LD;
     short v[NP * PLANE];
 
     // one 8-channel chunk
@@ -261,21 +271,30 @@ MVF_DEV uint64_t live_states(const AttnArgs &a, int b, int j0, int n, int lane)
     return __ballot(ok);
 }
 
-// This lane's chunks of a tile in flight: fetch() starts the loads of the rows `row_ptr(row)` (nullptr: zeros), commit() puts
-// them into the tile.  The loads of a tile are issued before the products of the one before it.
-template <int NP, int ROWS, int DP>
+// This lane's chunks of a tile in flight: fetch() starts the loads of the rows, which lie off(row) elements behind `base` (the
+// same in every lane; rows that are not valid(row) become zeros), commit() puts them into the tile.  The loads of a tile are
+// issued before the products of the one before it.  WIDE: 16-byte buffer loads, whose bounds check makes the zeros -- no branch,
+// so that all of a tile's loads are in flight at once; the host has checked that 32-bit byte offsets reach the rows of a tile.
+constexpr uint32_t kNowhere = 0x80000000u;
+template <int NP, int ROWS, int DP, bool WIDE>
 struct Flight {
+    typedef typename Elem<NP>::T T;
     static constexpr int CPR = DP / 8, CHUNKS = ROWS * CPR, N = (CHUNKS + NT - 1) / NT;
     Raw<NP> r[N];
-    template <typename F>
-    MVF_DEV void fetch(const AttnArgs &a, bool wide, F row_ptr)
+    template <typename V, typename F>
+    MVF_DEV void fetch(const T *base, int D, V valid, F off)
     {
+        __amdgpu_buffer_rsrc_t rs;
+        if constexpr (WIDE) rs = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, 0x7fffffff, 0x00027000);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = i * NT + threadIdx.x, row = c / CPR, ch = c - row * CPR;
-            const bool in = CHUNKS % NT == 0 || c < CHUNKS;
-            const typename Elem<NP>::T *p = in ? row_ptr(row) : nullptr;
-            r[i] = load8(p, ch * 8, a.D, wide, p != nullptr);
+            const bool in = (CHUNKS % NT == 0 || c < CHUNKS) && valid(row);
+            if constexpr (WIDE) {
+                r[i].load(rs, in && ch * 8 < D ? (uint32_t)(off(row) + ch * 8) * (uint32_t)sizeof(T) : kNowhere);
+            } else {
+                r[i] = load8(base + (in ? off(row) : 0), ch * 8, D, false, in);
+            }
         }
     }
     MVF_DEV void commit(Tile<NP, ROWS, DP> &t) const
@@ -287,6 +306,38 @@ struct Flight {
         }
     }
 };
+template <bool WIDE>
+struct Stride;                    // a stride, as wide as the offsets within a tile have to be
+template <>
+struct Stride<true> {
+    typedef int T;
+};
+template <>
+struct Stride<false> {
+    typedef int64_t T;
+};
+
+// Products whose left operands come from LDS: load(i) is issued AHEAD steps before mul(i, operand), and the order of the two
+// kinds is pinned (other instructions may cross), so that a wave waits for LDS once and not once per product.
+template <int NP>
+constexpr int kAhead = NP == 1 ? 4 : 1;
+#define MVF_PIN() __builtin_amdgcn_sched_barrier(0x2 | 0x4 | 0x10 | 0x200 | 0x400)     /* may cross: VALU, SALU, VMEM, LDS writes, transcendentals */
+template <int NP, int N, typename L, typename M>
+MVF_DEV void stream(L load, M mul)
+{
+    constexpr int A = kAhead<NP> < N ? kAhead<NP> : N;
+    Frag<NP> f[N];
+#pragma unroll
+    for (int i = 0; i < A; ++i) f[i] = load(i);
+    MVF_PIN();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i + A < N) f[i + A] = load(i + A);
+        MVF_PIN();
+        mul(i, f[i]);
+        MVF_PIN();
+    }
+}
 
 // The tiles of states a workgroup walks: [j, end) in steps of BK, those without a state that counts left out.  The same in
 // every lane of the workgroup.
@@ -337,7 +388,7 @@ MVF_DEV Frag<NP> acc_frag(const f32x16 &x, int s)
     float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
-    return split8<NP>(y);
+    return split8<NP, false>(y);
 }
 
 // four consecutive channels d .. d + 3 of a row
@@ -376,141 +427,143 @@ MVF_DEV void store_cols(T *row, const f32x16 (&acc)[DT], float f, int D, bool wi
                    acc[t][4 * i + 3] * f);
 }
 
-// NP == 3: the products of a tile are summed on their own and then added to the running sum, so that its roundings are one per
-// tile and not one per matrix instruction (3,840 states: error 5e-6 -> 1e-6 of the result)
+// acc[d] += (32 channels d of the tile's rows r0 .. r0 + 31)^T x.  NP == 3: the products of a tile are summed on their own and
+// then added to the running sum, so that its roundings are one per tile and not one per matrix instruction (3,840 states:
+// error 5e-6 -> 1e-6 of the result).
 template <int NP, int DT, int ROWS, int DP>
 MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, const f32x16 &x, int lane)
 {
-    const Frag<NP> x0 = acc_frag<NP>(x, 0), x1 = acc_frag<NP>(x, 1);
+    const Frag<NP> xf[2] = {acc_frag<NP>(x, 0), acc_frag<NP>(x, 1)};
+    if constexpr (NP == 1) {
+        stream<NP, 2 * DT>([&](int i) { return t.cols(32 * (i % DT), r0 + 16 * (i / DT), lane); },
+                           [&](int i, const Frag<NP> &f) { acc[i % DT] = mma(f, xf[i / DT], acc[i % DT]); });
+    } else {
+        f32x16 y;
+        stream<NP, 2 * DT>([&](int i) { return t.cols(32 * (i / 2), r0 + 16 * (i % 2), lane); },
+                           [&](int i, const Frag<NP> &f) {
+                               y = mma(f, xf[i % 2], i % 2 ? y : f32x16{});
+                               if (i % 2) {
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-        if constexpr (NP == 1) {
-            acc[d] = mma(t.cols(32 * d, r0, lane), x0, acc[d]);
-            acc[d] = mma(t.cols(32 * d, r0 + 16, lane), x1, acc[d]);
-        } else {
-            f32x16 y = {};
-            y = mma(t.cols(32 * d, r0, lane), x0, y);
-            y = mma(t.cols(32 * d, r0 + 16, lane), x1, y);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] += y[i];
-        }
+                                   for (int e = 0; e < 16; ++e) acc[i / 2][e] += y[e];
+                               }
+                           });
     }
 }
 
 // ------------------------------------------------------------------------------------------------- forward
-// grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x QT x 32 rows)
-template <int NP, int DP, int BK, int QT>
+// grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x 32 rows).  Two tile buffers: the
+// loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile.
+template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
     constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
     constexpr float kSlack = 8.0f;            // the reference of the exponentials follows the maximum once it is 2^8 behind
-    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tk;
-    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tv;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tile_k[buffers(NP)], tile_v[buffers(NP)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
     int id = xcd_run(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int rw = (tile * 4 + wave) * QT * 32 + col;             // this lane's first row
+    const int r = (tile * 4 + wave) * 32 + col;                   // this lane's row
+    const bool live = r < a.R;
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
-    const bool wide = a.wide;
     Walk<BK> w(a, b, part, lane);
-    Flight<NP, BK, DP> fk, fv;
+    Flight<NP, BK, DP, WIDE> fk, fv;
+    const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
     auto fetch = [&] {
-        fk.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? kb + (int64_t)(w.j + row) * a.ks[1] : (const T *)nullptr; });
-        fv.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? vb + (int64_t)(w.j + row) * a.vs[1] : (const T *)nullptr; });
+        auto valid = [&](int row) { return ((uint32_t)(row & 32 ? w.bits >> 32 : w.bits) >> (row & 31)) & 1; };
+        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, valid, [&](int row) { return row * ks; });
+        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, valid, [&](int row) { return row * vs; });
     };
     if (w.live()) fetch();
-    Frag<NP> qf[QT][KS];
-    f32x16 o[QT][DT];
-    float m[QT], sub[QT], l[QT];              // reference and sum of the exponentials; sub: the reference, 0 while there is none
+    Frag<NP> qf[KS];
+    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
 #pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const int r = rw + 32 * q;
-        const T *row = (const T *)a.q + (r < a.R ? row_off(a.qs, b, r, hk, a.G) : 0);
+    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+    f32x16 o[DT];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qf[q][s] = load_frag<NP>(row, 16 * s + 8 * h, a.D, wide, r < a.R);
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[q][t] = f32x16{};
-        m[q] = -INFINITY;
-        sub[q] = l[q] = 0.0f;
-    }
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    float m = -INFINITY, sub = 0.0f, l = 0.0f;                    // reference and sum of the exponentials; sub: 0 while there is none
+    constexpr bool kTwo = buffers(NP) == 2;
+    int buf = 0;
+    auto commit = [&] {
+        fk.commit(tile_k[buf]);
+        fv.commit(tile_v[buf]);
+    };
+    if (kTwo && w.live()) commit();
     while (w.live()) {
         const uint64_t bits = w.bits;
+        const Tile<NP, BK, DP> &tk = tile_k[buf], &tv = tile_v[buf];
         __syncthreads();
-        fk.commit(tk);
-        fv.commit(tv);
-        __syncthreads();
+        if (!kTwo) {
+            commit();
+            __syncthreads();
+        }
         w.next(a);
         if (w.live()) fetch();
+        f32x16 s[KT];
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            f32x16 s[QT];
+        for (int t = 0; t < KT; ++t) s[t] = f32x16{};
+        stream<NP, KT * KS>([&](int i) { return tk.rows(32 * (i % KT), 16 * (i / KT), lane); },
+                            [&](int i, const Frag<NP> &f) { s[i % KT] = mma(f, qf[i / KT], s[i % KT]); });
+        if (bits != Walk<BK>::kFull) {
 #pragma unroll
-            for (int q = 0; q < QT; ++q) s[q] = f32x16{};
-#pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const Frag<NP> kf = tk.rows(32 * t, 16 * x, lane);
-#pragma unroll
-                for (int q = 0; q < QT; ++q) s[q] = mma(kf, qf[q][x], s[q]);
-            }
-            if (bits != Walk<BK>::kFull) {
+            for (int t = 0; t < KT; ++t) {
                 const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
 #pragma unroll
-                for (int q = 0; q < QT; ++q)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!((ok >> acc_row(i, 0)) & 1)) s[q][i] = -INFINITY;
+                for (int i = 0; i < 16; ++i)
+                    if (!((ok >> acc_row(i, 0)) & 1)) s[t][i] = -INFINITY;
             }
+        }
+        float mx = s[0][0];
 #pragma unroll
-            for (int q = 0; q < QT; ++q) {
-                float mx = s[q][0];
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[q][i]);
-                mx = other_half_max(mx) * a.c;
-                if (__any(mx > m[q] + kSlack)) {
-                    mx = fmaxf(mx, m[q]);
-                    const float f = __builtin_amdgcn_exp2f(m[q] - (mx == -INFINITY ? 0.0f : mx));
-                    m[q] = mx;
-                    sub[q] = mx == -INFINITY ? 0.0f : mx;
-                    l[q] *= f;
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = other_half_max(mx) * a.c;
+        if (__any(mx > m + kSlack)) {
+            mx = fmaxf(mx, m);
+            sub = mx == -INFINITY ? 0.0f : mx;
+            const float f = __builtin_amdgcn_exp2f(m - sub);
+            m = mx;
+            l *= f;
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[q][d][i] *= f;
-                }
-                float lt = 0.0f;
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        float lt = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[q][i] = __builtin_amdgcn_exp2f(fmaf(s[q][i], a.c, -sub[q]));
-                    lt += s[q][i];
-                }
-                l[q] += lt;
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.c, -sub));
+                lt += s[t][i];
             }
+        l += lt;
 #pragma unroll
-            for (int q = 0; q < QT; ++q) accumulate<NP>(o[q], tv, 32 * t, s[q], lane);
+        for (int t = 0; t < KT; ++t) accumulate<NP>(o, tv, 32 * t, s[t], lane);
+        if (kTwo) {
+            buf ^= 1;
+            if (w.live()) commit();
         }
     }
-#pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const int r = rw + 32 * q;
-        const float lq = other_half_sum(l[q]);
-        if (r >= a.R) continue;
-        if (a.splits > 1) {                                      // this part's reference, sum and unscaled output
-            const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
-            store_cols<DT>(a.part + y * a.D, o[q], 1.0f, a.D, (a.D & 3) == 0, h);
-            if (h == 0) {
-                a.part2[2 * y] = m[q];
-                a.part2[2 * y + 1] = lq;
-            }
-            continue;
+    l = other_half_sum(l);
+    if (!live) return;
+    if (a.splits > 1) {                                          // this part's reference, sum and unscaled output
+        const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+        store_cols<DT>(a.part + y * a.D, o, 1.0f, a.D, (a.D & 3) == 0, h);
+        if (h == 0) {
+            a.part2[2 * y] = m;
+            a.part2[2 * y + 1] = l;
         }
-        const float inv = lq == 0.0f ? 0.0f : 1.0f / lq;
-        store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o[q], inv, a.D, (a.D & 7) == 0, h);
-        if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = lq == 0.0f ? INFINITY : m[q] + __builtin_amdgcn_logf(lq);
+        return;
     }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, WIDE || (a.D & 7) == 0, h);
+    if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
 // ------------------------------------------------------------------------------------------------- backward
@@ -520,218 +573,212 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
 // grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
-template <int NP, int DP, int BK, int QT>
+template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
     constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
-    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tk;
-    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tv;
+    __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tile_k[buffers(NP)], tile_v[buffers(NP)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
     int id = xcd_run(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int rw = (tile * 4 + wave) * QT * 32 + col;
+    const int r = (tile * 4 + wave) * 32 + col;
+    const bool live = r < a.R, dwide = WIDE || (a.D & 7) == 0;
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
-    const bool wide = a.wide, dwide = (a.D & 7) == 0;
     Walk<BK> w(a, b, part, lane);
-    Flight<NP, BK, DP> fk, fv;
+    Flight<NP, BK, DP, WIDE> fk, fv;
+    const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
     auto fetch = [&] {
-        fk.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? kb + (int64_t)(w.j + row) * a.ks[1] : (const T *)nullptr; });
-        fv.fetch(a, wide, [&](int row) { return (w.bits >> row) & 1 ? vb + (int64_t)(w.j + row) * a.vs[1] : (const T *)nullptr; });
+        auto valid = [&](int row) { return ((uint32_t)(row & 32 ? w.bits >> 32 : w.bits) >> (row & 31)) & 1; };
+        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, valid, [&](int row) { return row * ks; });
+        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, valid, [&](int row) { return row * vs; });
     };
     if (w.live()) fetch();
-    Frag<NP> qf[QT][KS], gf[QT][KS];
-    f32x16 dq[QT][DT];
-    float delta[QT], lse[QT];
+    Frag<NP> qf[KS], gf[KS];
+    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
+    const int64_t dense = live ? dense_row(b, r, hk, a) : 0;
+    float delta = 0.0f;
 #pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const int r = rw + 32 * q;
-        const bool live = r < a.R;
-        const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
-        const int64_t dense = live ? dense_row(b, r, hk, a) : 0;
-        float de = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            qf[q][s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, wide, live);
-            const Raw<NP> g = load8((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
-            de = dot8(g, load8((const T *)a.o + dense, 16 * s + 8 * h, a.D, dwide, live), de);
-            gf[q][s] = g.frag();
-        }
-        delta[q] = other_half_sum(de);
-        lse[q] = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
-        if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta[q];
-#pragma unroll
-        for (int t = 0; t < DT; ++t) dq[q][t] = f32x16{};
+    for (int s = 0; s < KS; ++s) {
+        qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+        const Raw<NP> g = load8((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
+        delta = dot8(g, load8((const T *)a.o + dense, 16 * s + 8 * h, a.D, dwide, live), delta);
+        gf[s] = g.frag();
     }
+    delta = other_half_sum(delta);
+    const float lse = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
+    if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta;
+    f32x16 dq[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
+    constexpr bool kTwo = buffers(NP) == 2;
+    int buf = 0;
+    auto commit = [&] {
+        fk.commit(tile_k[buf]);
+        fv.commit(tile_v[buf]);
+    };
+    if (kTwo && w.live()) commit();
     while (w.live()) {
         const uint64_t bits = w.bits;
+        const Tile<NP, BK, DP> &tk = tile_k[buf], &tv = tile_v[buf];
         __syncthreads();
-        fk.commit(tk);
-        fv.commit(tv);
-        __syncthreads();
+        if (!kTwo) {
+            commit();
+            __syncthreads();
+        }
         w.next(a);
         if (w.live()) fetch();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            f32x16 s[QT], dp[QT];
-#pragma unroll
-            for (int q = 0; q < QT; ++q) s[q] = dp[q] = f32x16{};
-#pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const Frag<NP> kf = tk.rows(32 * t, 16 * x, lane), vf = tv.rows(32 * t, 16 * x, lane);
-#pragma unroll
-                for (int q = 0; q < QT; ++q) {
-                    s[q] = mma(kf, qf[q][x], s[q]);
-                    dp[q] = mma(vf, gf[q][x], dp[q]);
-                }
-            }
+            f32x16 s = {}, dp = {};
+            stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tv : tk).rows(32 * t, 16 * (i / 2), lane); },
+                               [&](int i, const Frag<NP> &f) {
+                                   if (i % 2) dp = mma(f, gf[i / 2], dp);
+                                   else s = mma(f, qf[i / 2], s);
+                               });
             // a state that does not count: its row of the tile is zero, so whatever dS holds for it adds nothing to dq --
             // but exp2(-lse) may be infinite there, so it is cleared
-            const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
             if (bits != Walk<BK>::kFull) {
-#pragma unroll
-                for (int q = 0; q < QT; ++q)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!((ok >> acc_row(i, 0)) & 1)) s[q][i] = -INFINITY;
-            }
-#pragma unroll
-            for (int q = 0; q < QT; ++q)
+                const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    s[q][i] = __builtin_amdgcn_exp2f(fmaf(s[q][i], a.c, -lse[q])) * (dp[q][i] - delta[q]);
+                    if (!((ok >> acc_row(i, 0)) & 1)) s[i] = -INFINITY;
+            }
 #pragma unroll
-            for (int q = 0; q < QT; ++q) accumulate<NP>(dq[q], tk, 32 * t, s[q], lane);
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * (dp[i] - delta);
+            accumulate<NP>(dq, tk, 32 * t, s, lane);
+        }
+        if (kTwo) {
+            buf ^= 1;
+            if (w.live()) commit();
         }
     }
-#pragma unroll
-    for (int q = 0; q < QT; ++q) {
-        const int r = rw + 32 * q;
-        if (r >= a.R) continue;
-        if (a.splits > 1) {
-            const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
-            store_cols<DT>(a.part + y * a.D, dq[q], a.scale, a.D, (a.D & 3) == 0, h);
-            continue;
-        }
-        store_cols<DT>((T *)a.dq + dense_row(b, r, hk, a), dq[q], a.scale, a.D, dwide, h);
+    if (!live) return;
+    if (a.splits > 1) {
+        const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+        store_cols<DT>(a.part + y * a.D, dq, a.scale, a.D, (a.D & 3) == 0, h);
+        return;
     }
+    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, dwide, h);
 }
 
-// grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x KT x 32 states).  Row tiles of q and
-// do are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS
-template <int NP, int DP, int BQ, int KT>
+// grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
+// are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS
+template <int NP, int DP, int BQ, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
     constexpr int KS = DP / 16, DT = DP / 32, QT = BQ / 32;
-    __shared__ __attribute__((aligned(16))) Tile<NP, BQ, DP> tq;
-    __shared__ __attribute__((aligned(16))) Tile<NP, BQ, DP> tg;
-    __shared__ __attribute__((aligned(16))) float sl[BQ], sd[BQ];
+    __shared__ __attribute__((aligned(16))) Tile<NP, BQ, DP> tile_q[buffers(NP)], tile_g[buffers(NP)];
+    __shared__ __attribute__((aligned(16))) float row_lse[buffers(NP)][BQ], row_delta[buffers(NP)][BQ];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
     int id = xcd_run(blockIdx.x, gridDim.x);
     const int tile = id % a.tiles;
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
-    const int jw = (tile * 4 + wave) * KT * 32 + col, n = states_of(a, b);
-    const bool wide = a.wide, dwide = (a.D & 7) == 0;
-    Frag<NP> kf[KT][KS], vf[KT][KS];
-    f32x16 dk[KT][DT], dv[KT][DT];
-    bool live[KT];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const int j = jw + 32 * t;
-        live[t] = j < n && (!a.mask || a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0);
-        const T *krow = (const T *)a.k + (live[t] ? (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)hk * a.ks[2] : 0);
-        const T *vrow = (const T *)a.v + (live[t] ? (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)hk * a.vs[2] : 0);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            kf[t][s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, wide, live[t]);
-            vf[t][s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, wide, live[t]);
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x16{};
-    }
-    const int r1 = tile * 4 * KT * 32 < n ? (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ) : 0;
+    const int j = (tile * 4 + wave) * 32 + col, n = states_of(a, b);
+    const bool dwide = WIDE || (a.D & 7) == 0;
+    const int r1 = tile * 128 < n ? (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ) : 0;
     int r0 = part * a.per * BQ;
-    Flight<NP, BQ, DP> fq, fg;
+    Flight<NP, BQ, DP, WIDE> fq, fg;
     float pl = 0.0f, pd = 0.0f;
+    const typename Stride<WIDE>::T qs1 = a.qs[1], qs2 = a.qs[2], gs1 = (int64_t)a.Hq * a.D, gs2 = a.D;
+    const float invG = 1.0f / (float)a.G;
     auto fetch = [&] {
-        fq.fetch(a, wide, [&](int row) { return r0 + row < a.R ? (const T *)a.q + row_off(a.qs, b, r0 + row, hk, a.G) : (const T *)nullptr; });
-        fg.fetch(a, dwide, [&](int row) { return r0 + row < a.R ? (const T *)a.go + dense_row(b, r0 + row, hk, a) : (const T *)nullptr; });
+        // row r0 + row is token i0 + i, head g of the group: (g0 + row) / G by a product, exact for the small numbers that come up
+        // (G <= kMaxGroup; half a unit away from every integer)
+        const int i0 = r0 / a.G, g0 = r0 - i0 * a.G;
+        auto valid = [&](int row) { return r0 + row < a.R; };
+        auto token = [&](int row) { return (int)(((float)(g0 + row) + 0.5f) * invG); };
+        const T *qb = (const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)hk * a.G * a.qs[2] + (int64_t)i0 * a.qs[1];
+        const T *gb = (const T *)a.go + (((int64_t)b * a.Lq + i0) * a.Hq + (int64_t)hk * a.G) * a.D;
+        fq.fetch(qb, a.D, valid, [&](int row) { const int i = token(row); return i * qs1 + (g0 + row - i * a.G) * qs2; });
+        fg.fetch(gb, a.D, valid, [&](int row) { const int i = token(row); return i * gs1 + (g0 + row - i * a.G) * gs2; });
         if (threadIdx.x < BQ) {
             const int r = r0 + threadIdx.x;
             pl = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;            // rows behind the last: P = 0
             pd = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.0f;
         }
     };
-    if (r0 < r1) fetch();
-    while (r0 < r1) {
-        __syncthreads();
-        fq.commit(tq);
-        fg.commit(tg);
+    constexpr bool kTwo = buffers(NP) == 2;
+    int buf = 0;
+    auto commit = [&] {
+        fq.commit(tile_q[buf]);
+        fg.commit(tile_g[buf]);
         if (threadIdx.x < BQ) {
-            sl[threadIdx.x] = pl;
-            sd[threadIdx.x] = pd;
+            row_lse[buf][threadIdx.x] = pl;
+            row_delta[buf][threadIdx.x] = pd;
         }
+    };
+    if (r0 < r1) fetch();
+    const bool live = j < n && (!a.mask || a.mask[(int64_t)b * a.ms[0] + (int64_t)j * a.ms[1]] != 0);
+    const T *krow = (const T *)a.k + (live ? (int64_t)b * a.ks[0] + (int64_t)j * a.ks[1] + (int64_t)hk * a.ks[2] : 0);
+    const T *vrow = (const T *)a.v + (live ? (int64_t)b * a.vs[0] + (int64_t)j * a.vs[1] + (int64_t)hk * a.vs[2] : 0);
+    Frag<NP> kf[KS], vf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        kf[s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, WIDE, live);
+        vf[s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, WIDE, live);
+    }
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dk[d] = dv[d] = f32x16{};
+    if (kTwo && r0 < r1) commit();
+    while (r0 < r1) {
+        const Tile<NP, BQ, DP> &tq = tile_q[buf], &tg = tile_g[buf];
+        const float *sl = row_lse[buf], *sd = row_delta[buf];
         __syncthreads();
+        if (!kTwo) {
+            commit();
+            __syncthreads();
+        }
         r0 += BQ;
         if (r0 < r1) fetch();
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
-            f32x16 s[KT], dp[KT];
-#pragma unroll
-            for (int t = 0; t < KT; ++t) s[t] = dp[t] = f32x16{};
-#pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const Frag<NP> qf = tq.rows(32 * u, 16 * x, lane), gf = tg.rows(32 * u, 16 * x, lane);
-#pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    s[t] = mma(qf, kf[t][x], s[t]);
-                    dp[t] = mma(gf, vf[t][x], dp[t]);
-                }
-            }
+            f32x16 s = {}, dp = {};
+            stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tg : tq).rows(32 * u, 16 * (i / 2), lane); },
+                               [&](int i, const Frag<NP> &f) {
+                                   if (i % 2) dp = mma(f, vf[i / 2], dp);
+                                   else s = mma(f, kf[i / 2], s);
+                               });
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 ls = *(const f32x4 *)&sl[32 * u + acc_row(4 * i, h)], de = *(const f32x4 *)&sd[32 * u + acc_row(4 * i, h)];
 #pragma unroll
-                for (int t = 0; t < KT; ++t)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        // (the column of a state that does not count is dropped at the end)
-                        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][4 * i + e], a.c, -ls[e]));
-                        s[t][4 * i + e] = p;
-                        dp[t][4 * i + e] = p * (dp[t][4 * i + e] - de[e]);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    // (the column of a state that does not count is dropped at the end)
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], a.c, -ls[e]));
+                    s[4 * i + e] = p;
+                    dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
+                }
             }
-#pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                accumulate<NP>(dv[t], tg, 32 * u, s[t], lane);
-                accumulate<NP>(dk[t], tq, 32 * u, dp[t], lane);
-            }
+            accumulate<NP>(dv, tg, 32 * u, s, lane);
+            accumulate<NP>(dk, tq, 32 * u, dp, lane);
+        }
+        if (kTwo) {
+            buf ^= 1;
+            if (r0 < r1) commit();
         }
     }
+    if (j >= a.Lk) return;
+    if (!live) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const int j = jw + 32 * t;
-        if (j >= a.Lk) continue;
-        if (!live[t]) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) dk[t][d] = dv[t][d] = f32x16{};
-        }
-        if (a.splits > 1) {
-            const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, y = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
-            const bool pw = (a.D & 3) == 0;
-            store_cols<DT>(a.part + y, dk[t], a.scale, a.D, pw, h);
-            store_cols<DT>(a.part + y + n1, dv[t], 1.0f, a.D, pw, h);
-            continue;
-        }
-        const int64_t y = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
-        store_cols<DT>((T *)a.dk + y, dk[t], a.scale, a.D, dwide, h);
-        store_cols<DT>((T *)a.dv + y, dv[t], 1.0f, a.D, dwide, h);
+        for (int d = 0; d < DT; ++d) dk[d] = dv[d] = f32x16{};
     }
+    if (a.splits > 1) {
+        const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, y = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
+        const bool pw = (a.D & 3) == 0;
+        store_cols<DT>(a.part + y, dk, a.scale, a.D, pw, h);
+        store_cols<DT>(a.part + y + n1, dv, 1.0f, a.D, pw, h);
+        return;
+    }
+    const int64_t y = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
+    store_cols<DT>((T *)a.dk + y, dk, a.scale, a.D, dwide, h);
+    store_cols<DT>((T *)a.dv + y, dv, 1.0f, a.D, dwide, h);
 }
 
 // ------------------------------------------------------------------------------------------------- joining parts
@@ -801,7 +848,7 @@ constexpr int kWant = 512;         // workgroups that fill the chip (two per CU)
 // enough to, with at least four tiles each, at most 64
 void split_of(int64_t blocks, int red, int &splits, int &per)
 {
-    int64_t s = blocks > 0 && blocks < kWant * 3 / 4 ? kWant / blocks : 1;
+    int64_t s = blocks > 0 && blocks < kWant / 2 ? kWant / blocks : 1;
     if (s > 64) s = 64;
     if (s > red / 4) s = red / 4;
     if (s < 1) s = 1;
@@ -810,32 +857,45 @@ void split_of(int64_t blocks, int red, int &splits, int &per)
     splits = red > 0 ? (red + per - 1) / per : 1;
 }
 
-// two 32-row tiles per wave halve the LDS reads per product; they fit the registers of one plane up to 64 channels
-constexpr bool two_tiles(int NP, int DP) { return NP == 1 && DP <= 64; }
+// states of a staged tile
+constexpr int tile_states(int NP, int DP) { return NP == 1 || DP <= 32 ? 64 : 32; }
+// rows of a staged tile of the dk / dv kernel
+constexpr int tile_rows(int NP, int DP) { return NP == 1 && DP <= 64 ? 64 : 32; }
+constexpr int kMaxGroup = 65536;
+
+// whether 16-byte loads fit: aligned rows, and 32-bit byte offsets within a tile of 64 rows or states
+bool wide_rows(const mvf_attn_desc &d)
+{
+    const int64_t align = d.dtype == MVF_DTYPE_BF16 ? 8 : 4, G = d.Hq / d.Hk, most = 0x7fffffffLL / 4 - 128;
+    if (d.D % 8 || G > kMaxGroup) return false;
+    for (int i = 0; i < 3; ++i)
+        if (d.q_stride[i] % align || d.k_stride[i] % align || d.v_stride[i] % align) return false;
+    if (((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) & 15) return false;
+    const int64_t *q = d.q_stride, *k = d.k_stride, *v = d.v_stride;
+    if (q[1] < 0 || q[2] < 0 || k[1] < 0 || v[1] < 0 || q[1] > most || q[2] > most || k[1] > most / 64 || v[1] > most / 64) return false;
+    // (64 rows reach over 63 / G + 2 tokens, and the G heads of one)
+    return (63 / G + 2) * q[1] + G * q[2] <= most && ((63 / G + 2) * d.Hq + G) * d.D <= most;
+}
 
 struct Plan {
+    bool wide;                               // 16-byte loads
     int NP, DP, BK, BQ;
-    int fq, qq, kk;                          // 32-row (32-state) tiles per wave: forward, dq, dkv
-    int ftiles, qtiles, ktiles;              // workgroups along the rows (states)
-    int fs, fper, qs, qper, ks, kper;        // parts of the reduction, and tiles of a part
+    int rtiles, ktiles;                      // workgroups along the rows, along the states
+    int fs, fper, ks, kper;                  // parts of the reduction and tiles of a part: over the states (forward, dq), over the rows
 };
 Plan plan_of(const mvf_attn_desc &d)
 {
     Plan p;
+    p.wide = wide_rows(d);
     p.NP = d.dtype == MVF_DTYPE_F32 ? 3 : 1;
     p.DP = d.D <= 32 ? 32 : d.D <= 64 ? 64 : d.D <= 96 ? 96 : 128;
-    p.BK = p.NP == 1 ? 64 : 32;
-    p.BQ = 32;
+    p.BK = tile_states(p.NP, p.DP);
+    p.BQ = tile_rows(p.NP, p.DP);
     const int R = d.Lq * (d.Hq / d.Hk);
     const int64_t bh = (int64_t)d.B * d.Hk;
-    p.fq = two_tiles(p.NP, p.DP) && bh * (R / 256) >= kWant ? 2 : 1;
-    p.qq = p.fq;
-    p.kk = two_tiles(p.NP, p.DP) && bh * (d.Lk / 256) >= kWant ? 2 : 1;
-    p.ftiles = (R + 128 * p.fq - 1) / (128 * p.fq);
-    p.qtiles = (R + 128 * p.qq - 1) / (128 * p.qq);
-    p.ktiles = (d.Lk + 128 * p.kk - 1) / (128 * p.kk);
-    split_of(bh * p.ftiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
-    split_of(bh * p.qtiles, (d.Lk + p.BK - 1) / p.BK, p.qs, p.qper);
+    p.rtiles = (R + 127) / 128;
+    p.ktiles = (d.Lk + 127) / 128;
+    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
     split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, p.ks, p.kper);
     return p;
 }
@@ -854,14 +914,8 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
     AttnArgs a = {};
     a.q = d.q; a.k = d.k; a.v = d.v;
     a.mask = d.key_mask; a.lens = d.kv_lens;
-    bool wide = d.D % 8 == 0;
-    const int64_t align = p.NP == 1 ? 8 : 4;             // elements in 16 bytes
-    for (int i = 0; i < 3; ++i) {
-        a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i];
-        wide = wide && a.qs[i] % align == 0 && a.ks[i] % align == 0 && a.vs[i] % align == 0;
-    }
-    wide = wide && !(((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) & 15);
-    a.wide = wide;
+    for (int i = 0; i < 3; ++i) { a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i]; }
+    a.wide = p.wide;
     a.ms[0] = d.mask_stride[0]; a.ms[1] = d.mask_stride[1];
     a.B = d.B; a.Lq = d.Lq; a.Lk = d.Lk; a.Hq = d.Hq; a.Hk = d.Hk; a.D = d.D;
     a.G = d.Hq / d.Hk;
@@ -872,36 +926,25 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
 }
 
 template <int NP, int DP>
-void launch_fwd(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
+void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
 {
-    constexpr int BK = NP == 1 ? 64 : 32;
-    if constexpr (two_tiles(NP, DP))
-        if (tiles == 2) {
-            hipLaunchKernelGGL((k_attn_fwd<NP, DP, BK, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-            return;
-        }
-    hipLaunchKernelGGL((k_attn_fwd<NP, DP, BK, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    constexpr int BT = tile_states(NP, DP);
+    if (a.wide) hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
-void launch_dq(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
+void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
 {
-    constexpr int BK = NP == 1 ? 64 : 32;
-    if constexpr (two_tiles(NP, DP))
-        if (tiles == 2) {
-            hipLaunchKernelGGL((k_attn_dq<NP, DP, BK, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-            return;
-        }
-    hipLaunchKernelGGL((k_attn_dq<NP, DP, BK, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    constexpr int BT = tile_states(NP, DP);
+    if (a.wide) hipLaunchKernelGGL((k_attn_dq<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_dq<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
-void launch_dkv(const AttnArgs &a, int tiles, int64_t blocks, hipStream_t st)
+void launch_dkv(const AttnArgs &a, int64_t blocks, hipStream_t st)
 {
-    if constexpr (two_tiles(NP, DP))
-        if (tiles == 2) {
-            hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32, 2>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-            return;
-        }
-    hipLaunchKernelGGL((k_attn_dkv<NP, DP, 32, 1>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    constexpr int BT = tile_rows(NP, DP);
+    if (a.wide) hipLaunchKernelGGL((k_attn_dkv<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_dkv<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int MODE>
 void launch_join(const AttnArgs &a, int NP, int64_t rows, hipStream_t st)
@@ -952,12 +995,12 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     const int64_t rows = (int64_t)d->B * d->Hq * d->Lq;
     a.out = out;
     a.lse = lse;
-    a.tiles = p.ftiles; a.splits = p.fs; a.per = p.fper;
+    a.tiles = p.rtiles; a.splits = p.fs; a.per = p.fper;
     a.part = (float *)workspace;
     a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
-    MVF_ATTN_PICK(launch_fwd, p, a, p.fq, (int64_t)d->B * d->Hk * p.ftiles * p.fs, st);
+    MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
     if (p.fs > 1) launch_join<0>(a, p.NP, rows, st);
     return hip_check_launch();
 }
@@ -968,7 +1011,7 @@ size_t mvf_cross_attention_bwd_workspace_bytes(const mvf_attn_desc *d)
     const Plan p = plan_of(*d);
     const int64_t rows = (int64_t)d->B * d->Hq * d->Lq, states = (int64_t)d->B * d->Hk * d->Lk;
     const int64_t delta = (rows + 3) / 4 * 4;
-    const int64_t pq = p.qs > 1 ? p.qs * rows * d->D : 0, pk = p.ks > 1 ? 2 * p.ks * states * d->D : 0;
+    const int64_t pq = p.fs > 1 ? p.fs * rows * d->D : 0, pk = p.ks > 1 ? 2 * p.ks * states * d->D : 0;
     return (size_t)((delta + (pq > pk ? pq : pk)) * 4);
 }
 
@@ -991,13 +1034,13 @@ int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_BWD, st, tensor_bytes(*d, 4 * rows + 4 * states));
     if (d->Lq > 0) {
-        a.tiles = p.qtiles; a.splits = p.qs; a.per = p.qper;
-        MVF_ATTN_PICK(launch_dq, p, a, p.qq, (int64_t)d->B * d->Hk * p.qtiles * p.qs, st);
-        if (p.qs > 1) launch_join<1>(a, p.NP, rows, st);
+        a.tiles = p.rtiles; a.splits = p.fs; a.per = p.fper;
+        MVF_ATTN_PICK(launch_dq, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
+        if (p.fs > 1) launch_join<1>(a, p.NP, rows, st);
     }
     if (d->Lk > 0 && g_k) {
         a.tiles = p.ktiles; a.splits = p.ks; a.per = p.kper;
-        MVF_ATTN_PICK(launch_dkv, p, a, p.kk, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
+        MVF_ATTN_PICK(launch_dkv, p, a, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
         if (p.ks > 1) launch_join<2>(a, p.NP, 2 * states, st);
     }
     return hip_check_launch();
