@@ -14,8 +14,8 @@
 // altogether at far positions: half a step of 300,000 is a sixtieth of a radian.)
 //
 // Bound by memory: 2 passes over the rows forward, 3 backward.  A group of lanes owns a token, so the sines and cosines are
-// formed once for all its heads; a lane owns the same pairs of every head, loads them with 8- or 16-byte accesses, and the sum
-// of squares is a butterfly over the group.  All arithmetic is fp32; bf16 is rounded once, at the store.
+// formed once for all its heads; a lane owns the same pairs of every head, loads them in runs of four, two or one, and the sum
+// of squares is a butterfly over the group (DPP), for all heads in flight at once.  All arithmetic is fp32; bf16 is rounded once, at the store.
 #include "mvf_common.hpp"
 
 using namespace mvf;
@@ -23,11 +23,14 @@ using namespace mvf;
 namespace {
 
 constexpr int NT = 256;
-constexpr int HB = 4;             // heads in flight per lane
+constexpr int HB = 4, HG = 2;     // heads in flight per lane, forward and backward (two tensors)
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+// runs of N channels, as aligned as their elements are
+template <typename T, int N>
+struct Run {
+    typedef T V __attribute__((ext_vector_type(N)));
+    typedef V U __attribute__((aligned(sizeof(T))));
+};
 
 struct Side {
     const void *x, *gy;
@@ -46,8 +49,8 @@ struct NormArgs {
     int D, axes, rot, ra;
     int units, rotu;              // units (of PV pairs) of a row; the rotated ones
     int lpr;                      // lanes of a row: power of two >= units
-    int pos64;
-    float eps;
+    int pos64, ragged;
+    float eps, invD;
 };
 
 // sine and cosine of `turn` / 2^64 of a full turn
@@ -75,10 +78,11 @@ MVF_DEV void sincos_turn(uint64_t turn, float &s, float &c)
 // otherwise two runs of PV from c0 and c1 (channels that are not rotated have no partner: any pairing of them will do)
 template <int PV, bool NB>
 struct Unit {
-    int c0, c1;
-    bool live, rot;
+    int c0, c1;                   // first channels of the two runs (NB: c1 = c0 + PV); 0 where there is none
+    bool live, live1, rot;        // whether the lane has a unit, and that a second run
     float sn[PV], cs[PV];
-    MVF_DEV int channel(int i) const { return NB ? (i < PV ? c0 + 2 * i : c0 + 2 * (i - PV) + 1) : (i < PV ? c0 + i : c1 + i - PV); }
+    MVF_DEV int channel(int i) const { return NB ? c0 + (i < PV ? 2 * i : 2 * (i - PV) + 1) : (i < PV ? c0 + i : c1 + i - PV); }
+    MVF_DEV bool has(int i) const { return NB ? (channel(i) - c0 < PV ? live : live1) : (i < PV ? live : live1); }
 };
 
 template <int PV, bool NB>
@@ -90,11 +94,14 @@ MVF_DEV Unit<PV, NB> unit_of(const NormArgs &a, int u)
     if (t.rot) {
         const int j = u * PV, per = a.ra / 2, ax = j / per, jj = j - ax * per;
         t.c0 = ax * a.ra + (NB ? 2 * jj : jj);
-        t.c1 = t.c0 + per;
+        t.c1 = NB ? t.c0 + PV : t.c0 + per;
     } else {
         t.c0 = a.rot + (u - a.rotu) * 2 * PV;
         t.c1 = t.c0 + PV;
     }
+    t.live1 = t.live && t.c1 < a.D;
+    if (!t.live) t.c0 = 0;
+    if (!t.live1) t.c1 = 0;
 #pragma unroll
     for (int i = 0; i < PV; ++i) { t.sn[i] = 0.0f; t.cs[i] = 1.0f; }
     return t;
@@ -110,72 +117,88 @@ MVF_DEV void angles(Unit<PV, NB> &t, const NormArgs &a, const Side &s, int u, in
     for (int i = 0; i < PV; ++i) sincos_turn((uint64_t)p * a.freq[jj + i], t.sn[i], t.cs[i]);
 }
 
-template <int N>
-MVF_DEV void load_run(const float *p, float *v)
+template <int N, typename T>
+MVF_DEV void load_run(const T *p, float (&v)[N])
 {
-    static_assert(N == 4, "");
-    const f32x4 x = *(const f32x4 *)p;
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = x[i];
-}
-template <int N>
-MVF_DEV void load_run(const __bf16 *p, float *v)
-{
-    static_assert(N == 4, "");
-    const bf16x4 x = *(const bf16x4 *)p;
+    const typename Run<T, N>::V x = *(const typename Run<T, N>::U *)p;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)x[i];
 }
-MVF_DEV void store_run(float *p, const float *v) { *(f32x4 *)p = f32x4{v[0], v[1], v[2], v[3]}; }
-MVF_DEV void store_run(__bf16 *p, const float *v)
+template <int N, typename T>
+MVF_DEV void store_run(T *p, const float (&v)[N], bool in)
 {
-    bf16x4 x;
+    if (!in) return;
+    typename Run<T, N>::V x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (__bf16)v[i];
-    *(bf16x4 *)p = x;
+    for (int i = 0; i < N; ++i) x[i] = (T)v[i];
+    *(typename Run<T, N>::U *)p = x;
+}
+// the unit's 2 PV values of a row, as pairs (v[i], v[PV + i]): two runs of PV channels, each whole inside the row or not there.
+// Runs that are not there are loaded from channel 0 and cleared (`ragged`: some lane has one), so that no load waits in a branch
+template <int PV, bool NB, typename T>
+MVF_DEV void load_unit(const T *row, const Unit<PV, NB> &t, bool ragged, float (&v)[2 * PV])
+{
+    float r[2][PV];
+    load_run<PV>(row + t.c0, r[0]);
+    load_run<PV>(row + t.c1, r[1]);
+    if (ragged) {
+#pragma unroll
+        for (int i = 0; i < PV; ++i) {
+            r[0][i] = t.live ? r[0][i] : 0.0f;
+            r[1][i] = t.live1 ? r[1][i] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+        v[i] = NB ? r[2 * i / PV][2 * i % PV] : r[0][i];
+        v[PV + i] = NB ? r[(2 * i + 1) / PV][(2 * i + 1) % PV] : r[1][i];
+    }
+}
+template <int PV, bool NB, typename T>
+MVF_DEV void store_unit(T *row, const Unit<PV, NB> &t, const float (&v)[2 * PV], bool in)
+{
+    float r[2][PV];
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+        r[0][i] = NB ? v[(i & 1) * PV + i / 2] : v[i];
+        r[1][i] = NB ? v[((PV + i) & 1) * PV + (PV + i) / 2] : v[PV + i];
+    }
+    store_run<PV>(row + t.c0, r[0], in && t.live);
+    store_run<PV>(row + t.c1, r[1], in && t.live1);
 }
 
-// the unit's 2 PV values of a row, as pairs (v[i], v[PV + i])
-template <int PV, bool NB, typename T>
-MVF_DEV void load_unit(const T *row, const Unit<PV, NB> &t, int D, float (&v)[2 * PV])
+template <int CTRL>
+MVF_DEV float dpp(float x) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true)); }
+MVF_DEV float halves_sum(float x)
 {
-    if constexpr (PV == 1) {
-        v[0] = t.live && t.channel(0) < D ? (float)row[t.channel(0)] : 0.0f;
-        v[1] = t.live && t.channel(1) < D ? (float)row[t.channel(1)] : 0.0f;
-    } else {
-        float a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
-        if (t.live) {
-            load_run<4>(row + t.c0, a);
-            load_run<4>(row + (NB ? t.c0 + 4 : t.c1), b);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = NB ? (i < 2 ? a[2 * i & 3] : b[2 * i & 3]) : a[i];
-            v[4 + i] = NB ? (i < 2 ? a[(2 * i + 1) & 3] : b[(2 * i + 1) & 3]) : b[i];
-        }
-    }
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
-template <int PV, bool NB, typename T>
-MVF_DEV void store_unit(T *row, const Unit<PV, NB> &t, int D, const float (&v)[2 * PV])
+MVF_DEV float rows_sum(float x)
 {
-    if (!t.live) return;
-    if constexpr (PV == 1) {
-        if (t.channel(0) < D) row[t.channel(0)] = (T)v[0];
-        if (t.channel(1) < D) row[t.channel(1)] = (T)v[1];
-    } else if constexpr (NB) {
-        const float a[4] = {v[0], v[4], v[1], v[5]}, b[4] = {v[2], v[6], v[3], v[7]};
-        store_run(row + t.c0, a);
-        store_run(row + t.c0 + 4, b);
-    } else {
-        const float a[4] = {v[0], v[1], v[2], v[3]}, b[4] = {v[4], v[5], v[6], v[7]};
-        store_run(row + t.c0, a);
-        store_run(row + t.c1, b);
-    }
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
-MVF_DEV float group_sum(float x, int lpr)
+// sums over the aligned groups of `lpr` lanes, in every lane of the group (N of them side by side)
+template <int N>
+MVF_DEV void group_sum(float (&x)[N], int lpr)
 {
-    for (int m = lpr >> 1; m > 0; m >>= 1) x += __shfl_xor(x, m, 64);
-    return x;
+#define MVF_EACH(expr)           \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) x[k] = (expr)
+    if (lpr > 1) MVF_EACH(x[k] + dpp<0xB1>(x[k]));        // quad_perm [1,0,3,2]
+    if (lpr > 2) MVF_EACH(x[k] + dpp<0x4E>(x[k]));        // quad_perm [2,3,0,1]
+    if (lpr > 4) MVF_EACH(x[k] + dpp<0x141>(x[k]));       // row_half_mirror: the other quad of eight lanes
+    if (lpr > 8) MVF_EACH(x[k] + dpp<0x140>(x[k]));       // row_mirror: the other half of sixteen
+    if (lpr > 16) MVF_EACH(rows_sum(x[k]));
+    if (lpr > 32) MVF_EACH(halves_sum(x[k]));
+#undef MVF_EACH
+}
+// 1 / sqrt(x), also of denormals
+MVF_DEV float inv_sqrt(float x)
+{
+    const bool tiny = x < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? x * 0x1p+100f : x);
+    return tiny ? r * 0x1p+50f : r;
 }
 
 template <typename T, int PV, bool NB>
@@ -195,36 +218,33 @@ __global__ void __launch_bounds__(NT) k_qk_norm_fwd(const NormArgs a)
     float w[2 * PV];
 #pragma unroll
     for (int i = 0; i < 2 * PV; ++i) w[i] = 1.0f;
-    if (s.w) load_unit<PV, NB>(s.w, t, a.D, w);
+    if (s.w) load_unit<PV, NB>(s.w, t, a.ragged, w);
     const T *x0 = (const T *)s.x + b * s.s[0] + l * s.s[1];
     T *y0 = (T *)s.y + tok * s.H * a.D;
     const int h1 = min(s.H, (ch + 1) * s.hg);
     for (int h0 = ch * s.hg; h0 < h1; h0 += HB) {
-        float v[HB][2 * PV];
+        // (heads behind the last are read as the last again and not stored: no branch, so that the loads go out together)
+        float v[HB][2 * PV], r[HB];
+#pragma unroll
+        for (int k = 0; k < HB; ++k) load_unit<PV, NB>(x0 + (int64_t)min(h0 + k, h1 - 1) * s.s[2], t, a.ragged, v[k]);
 #pragma unroll
         for (int k = 0; k < HB; ++k) {
-            if (h0 + k < h1) {
-                load_unit<PV, NB>(x0 + (int64_t)(h0 + k) * s.s[2], t, a.D, v[k]);
-            } else {
+            r[k] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 2 * PV; ++i) v[k][i] = 0.0f;
-            }
+            for (int i = 0; i < 2 * PV; ++i) r[k] = fmaf(v[k][i], v[k][i], r[k]);
         }
+        group_sum(r, a.lpr);
 #pragma unroll
         for (int k = 0; k < HB; ++k) {
-            // (the butterfly runs for heads behind the last too, on zeros: no branch, so that the rows stay in registers)
-            float q = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 2 * PV; ++i) q = fmaf(v[k][i], v[k][i], q);
-            const float r = 1.0f / sqrtf(group_sum(q, a.lpr) / (float)a.D + a.eps);
+            const float q = inv_sqrt(fmaf(r[k], a.invD, a.eps));
             float y[2 * PV];
 #pragma unroll
             for (int i = 0; i < PV; ++i) {
-                const float p = v[k][i] * r * w[i], n = v[k][PV + i] * r * w[PV + i];
+                const float p = v[k][i] * q * w[i], n = v[k][PV + i] * q * w[PV + i];
                 y[i] = fmaf(p, t.cs[i], -(n * t.sn[i]));
                 y[PV + i] = fmaf(p, t.sn[i], n * t.cs[i]);
             }
-            if (h0 + k < h1) store_unit<PV, NB>(y0 + (int64_t)(h0 + k) * a.D, t, a.D, y);
+            store_unit<PV, NB>(y0 + (int64_t)(h0 + k) * a.D, t, y, h0 + k < h1);
         }
     }
 }
@@ -242,7 +262,7 @@ __global__ void __launch_bounds__(NT) k_qk_norm_bwd(const NormArgs a)
     float w[2 * PV], dw[2 * PV];
 #pragma unroll
     for (int i = 0; i < 2 * PV; ++i) { w[i] = 1.0f; dw[i] = 0.0f; }
-    if (s.w) load_unit<PV, NB>(s.w, t, a.D, w);
+    if (s.w) load_unit<PV, NB>(s.w, t, a.ragged, w);
     for (int64_t g = blk * gpb + threadIdx.x / a.lpr; g < s.groups; g += s.blocks * gpb) {
         const int64_t tok = g / s.chunks;
         const int ch = (int)(g - tok * s.chunks);
@@ -252,43 +272,41 @@ __global__ void __launch_bounds__(NT) k_qk_norm_bwd(const NormArgs a)
         const T *g0 = (const T *)s.gy + tok * s.H * a.D;
         T *y0 = (T *)s.y + tok * s.H * a.D;
         const int h1 = min(s.H, (ch + 1) * s.hg);
-        for (int h0 = ch * s.hg; h0 < h1; h0 += HB) {
-            float v[HB][2 * PV], e[HB][2 * PV];
+        for (int h0 = ch * s.hg; h0 < h1; h0 += HG) {
+            float v[HG][2 * PV], f[HG][2 * PV], sum[2 * HG];
 #pragma unroll
-            for (int k = 0; k < HB; ++k) {
-                if (h0 + k < h1) {
-                    load_unit<PV, NB>(x0 + (int64_t)(h0 + k) * s.s[2], t, a.D, v[k]);
-                    load_unit<PV, NB>(g0 + (int64_t)(h0 + k) * a.D, t, a.D, e[k]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2 * PV; ++i) v[k][i] = e[k][i] = 0.0f;
-                }
+            for (int k = 0; k < HG; ++k) {
+                const int64_t hk = min(h0 + k, h1 - 1);
+                load_unit<PV, NB>(x0 + hk * s.s[2], t, a.ragged, v[k]);
+                load_unit<PV, NB>(g0 + hk * a.D, t, a.ragged, f[k]);
             }
 #pragma unroll
-            for (int k = 0; k < HB; ++k) {
-                float q = 0.0f, d = 0.0f;
-                float f[2 * PV];                                // u = R(-pos) dy
+            for (int k = 0; k < HG; ++k) {
+                sum[2 * k] = sum[2 * k + 1] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PV; ++i) {
-                    f[i] = fmaf(e[k][i], t.cs[i], e[k][PV + i] * t.sn[i]);
-                    f[PV + i] = fmaf(e[k][PV + i], t.cs[i], -(e[k][i] * t.sn[i]));
+                for (int i = 0; i < PV; ++i) {                  // u = R(-pos) dy
+                    const float e0 = f[k][i], e1 = f[k][PV + i];
+                    f[k][i] = fmaf(e0, t.cs[i], e1 * t.sn[i]);
+                    f[k][PV + i] = fmaf(e1, t.cs[i], -(e0 * t.sn[i]));
                 }
 #pragma unroll
                 for (int i = 0; i < 2 * PV; ++i) {
-                    q = fmaf(v[k][i], v[k][i], q);
-                    d = fmaf(f[i] * w[i], v[k][i], d);
+                    sum[2 * k] = fmaf(v[k][i], v[k][i], sum[2 * k]);
+                    sum[2 * k + 1] = fmaf(f[k][i] * w[i], v[k][i], sum[2 * k + 1]);
                 }
-                q = group_sum(q, a.lpr);
-                d = group_sum(d, a.lpr);
-                const float r = 1.0f / sqrtf(q / (float)a.D + a.eps);
-                const float z = d * r * r * r / (float)a.D;
+            }
+            group_sum(sum, a.lpr);
+#pragma unroll
+            for (int k = 0; k < HG; ++k) {
+                const bool in = h0 + k < h1;
+                const float r = inv_sqrt(fmaf(sum[2 * k], a.invD, a.eps)), z = sum[2 * k + 1] * r * r * r * a.invD, rw = in ? r : 0.0f;
                 float y[2 * PV];
 #pragma unroll
                 for (int i = 0; i < 2 * PV; ++i) {
-                    dw[i] = fmaf(f[i] * v[k][i], r, dw[i]);
-                    y[i] = fmaf(f[i] * w[i], r, -(v[k][i] * z));
+                    dw[i] = fmaf(f[k][i] * v[k][i], rw, dw[i]);
+                    y[i] = fmaf(f[k][i] * w[i], r, -(v[k][i] * z));
                 }
-                if (h0 + k < h1) store_unit<PV, NB>(y0 + (int64_t)(h0 + k) * a.D, t, a.D, y);
+                store_unit<PV, NB>(y0 + (int64_t)(h0 + k) * a.D, t, y, in);
             }
         }
     }
@@ -302,8 +320,7 @@ __global__ void __launch_bounds__(NT) k_qk_norm_bwd(const NormArgs a)
         for (int i = 0; i < 2 * PV; ++i) {
             float x = 0.0f;
             for (int k = threadIdx.x; k < NT; k += a.lpr) x += fold[i][k];
-            const int c = t.channel(i);
-            if (c < a.D) p[c] = x;
+            if (t.has(i)) p[t.channel(i)] = x;
         }
     }
 }
@@ -318,8 +335,10 @@ __global__ void __launch_bounds__(NT) k_qk_norm_dw(const float *p0, const float 
     if (!o) return;
     const int c = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
     float x = 0.0f;
-    if (c < D)
+    if (c < D) {
+#pragma unroll 8
         for (int i = k; i < n; i += 16) x += p[(int64_t)i * D + c];
+    }
     fold[k][threadIdx.x & 15] = x;
     __syncthreads();
     if (k == 0 && c < D) {
@@ -330,7 +349,7 @@ __global__ void __launch_bounds__(NT) k_qk_norm_dw(const float *p0, const float 
     }
 }
 
-constexpr int kWant = 2048, kBwdBlocks = 1024;     // workgroups: enough to fill the chip; rows of partial weight gradients
+constexpr int kWant = 1024, kBwdBlocks = 1024;     // workgroups: enough to fill the chip; rows of partial weight gradients
 
 bool bad_desc(const mvf_qk_norm_desc *d)
 {
@@ -342,23 +361,22 @@ bool bad_desc(const mvf_qk_norm_desc *d)
     return (int64_t)d->B * d->Lq * d->Hq > most || (int64_t)d->B * d->Lk * d->Hk > most;
 }
 
-// kernel arguments and which variant: returns PV (4 where every access of a unit is an aligned run of four channels, else 1)
+// kernel arguments and which variant: returns PV, the longest run of channels (4, 2, 1) that the blocks and the rest are made of
 int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
 {
     a = {};
     a.D = d.D; a.axes = d.axes; a.rot = d.rot; a.ra = d.rot / d.axes;
     a.pos64 = d.pos64;
     a.eps = d.eps;
+    a.invD = 1.0f / (float)d.D;
     for (int j = 0; j < a.ra / 2; ++j) a.freq[j] = d.freq[j];
-    bool wide = a.ra % 8 == 0 && (d.D - d.rot) % 8 == 0;
-    for (int i = 0; i < 3; ++i) wide = wide && d.q_stride[i] % 4 == 0 && d.k_stride[i] % 4 == 0;
-    const uintptr_t bits = (uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.q_weight | (uintptr_t)d.k_weight;
-    wide = wide && !(bits & 15);
-    const int PV = wide ? 4 : 1;
+    auto fits = [&](int n) { return a.ra / 2 % n == 0 && (d.D - d.rot) % n == 0; };
+    const int PV = fits(4) ? 4 : fits(2) ? 2 : 1;
     a.rotu = d.rot / 2 / PV;
     a.units = a.rotu + (d.D - d.rot + 2 * PV - 1) / (2 * PV);
     a.lpr = 1;
     while (a.lpr < a.units) a.lpr *= 2;
+    a.ragged = a.units < a.lpr || (d.D - d.rot) % (2 * PV);
     for (int i = 0; i < 2; ++i) {
         Side &s = a.side[i];
         s.x = i ? d.k : d.q;
@@ -377,7 +395,10 @@ int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
         s.chunks = (s.H + s.hg - 1) / s.hg;
         s.groups = tokens * s.chunks;
         s.blocks = (s.groups + gpb - 1) / gpb;
-        if (bwd && s.blocks > kBwdBlocks) s.blocks = kBwdBlocks;
+        if (bwd) {                                             // rows of partial weight gradients: half of the workgroups, 256 .. 1,024
+            const int64_t most = s.blocks / 2 < 256 ? 256 : s.blocks / 2 > kBwdBlocks ? kBwdBlocks : s.blocks / 2;
+            if (s.blocks > most) s.blocks = most;
+        }
     }
     return PV;
 }
@@ -389,10 +410,15 @@ int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
     } while (0)
 #define MVF_NORM_PICK(fn)                                                                       \
     do {                                                                                        \
-        if (esz == 4 && PV == 4) MVF_NORM_LAUNCH(fn, float, 4);                                 \
-        else if (esz == 4) MVF_NORM_LAUNCH(fn, float, 1);                                       \
-        else if (PV == 4) MVF_NORM_LAUNCH(fn, __bf16, 4);                                       \
-        else MVF_NORM_LAUNCH(fn, __bf16, 1);                                                    \
+        if (esz == 4) {                                                                         \
+            if (PV == 4) MVF_NORM_LAUNCH(fn, float, 4);                                         \
+            else if (PV == 2) MVF_NORM_LAUNCH(fn, float, 2);                                    \
+            else MVF_NORM_LAUNCH(fn, float, 1);                                                 \
+        } else {                                                                                \
+            if (PV == 4) MVF_NORM_LAUNCH(fn, __bf16, 4);                                        \
+            else if (PV == 2) MVF_NORM_LAUNCH(fn, __bf16, 2);                                   \
+            else MVF_NORM_LAUNCH(fn, __bf16, 1);                                                \
+        }                                                                                       \
     } while (0)
 
 }  // namespace
