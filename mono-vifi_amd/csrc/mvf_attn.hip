@@ -566,6 +566,159 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
     if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// The same for at most 32 rows (a few queries, or one with the heads of its group): four row tiles would leave three waves of a
+// workgroup idle, so here the waves share the rows and divide the states, 32 each in turn, every wave on its own: keys go from
+// memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
+// wave's own, the next 32 states are in flight meanwhile, and no barrier until the four partial results are joined in LDS.
+// Bound by the bytes of keys and values.  (5 rows against 40,001 fp32 states of 6 heads of 80: 92 us by row tiles.)
+template <int NP, int DP, bool WIDE>
+__global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
+{
+    typedef typename Elem<NP>::T T;
+    typedef Tile<NP, 32, DP> VT;
+    constexpr int KS = DP / 16, DT = DP / 32, LO = DP + 4, NV = 32 * (DP / 8) / 64;
+    constexpr size_t kTiles = 4 * sizeof(VT), kOut = 4 * 32 * LO * sizeof(float);
+    __shared__ __attribute__((aligned(16))) char mem[kTiles > kOut ? kTiles : kOut];
+    __shared__ float wave_m[4][32], wave_l[4][32];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    const int id = xcd_run(blockIdx.x, gridDim.x), part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
+    VT &tv = ((VT *)mem)[wave];
+    const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
+    const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
+    const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
+    const int n = states_of(a, b), end = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * 128);
+    int j = part * a.per * 128 + wave * 32;
+    uint32_t bits = 0;
+    auto settle = [&] {                                           // on to 32 states of which one counts
+        for (; j < end; j += 128) {
+            bits = (uint32_t)live_states(a, b, j, n, lane);
+            if (bits) return;
+        }
+    };
+    Raw<NP> rk[KS], rv[NV];
+    auto fetch = [&] {
+        const T *kt = kb + (int64_t)j * a.ks[1], *vt = vb + (int64_t)j * a.vs[1];
+        const bool mine = (bits >> col) & 1;
+        if constexpr (WIDE) {
+            const __amdgpu_buffer_rsrc_t sk = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(kt), (short)0, 0x7fffffff, 0x00027000);
+            const __amdgpu_buffer_rsrc_t sv = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(vt), (short)0, 0x7fffffff, 0x00027000);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const int d = 16 * s + 8 * h;
+                rk[s].load(sk, mine && d < a.D ? (uint32_t)(col * ks + d) * (uint32_t)sizeof(T) : kNowhere);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = i * 64 + lane, row = c / (DP / 8), d = (c - row * (DP / 8)) * 8;
+                rv[i].load(sv, ((bits >> row) & 1) && d < a.D ? (uint32_t)(row * vs + d) * (uint32_t)sizeof(T) : kNowhere);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) rk[s] = load8(kt + (mine ? col * ks : 0), 16 * s + 8 * h, a.D, false, mine);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = i * 64 + lane, row = c / (DP / 8), d = (c - row * (DP / 8)) * 8;
+                const bool in = (bits >> row) & 1;
+                rv[i] = load8(vt + (in ? row * vs : 0), d, a.D, false, in);
+            }
+        }
+    };
+    settle();
+    if (j < end) fetch();
+    const bool live = col < a.R;
+    const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, col, hk, a.G) : 0);
+    Frag<NP> qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+    f32x16 o[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+    while (j < end) {
+        const uint32_t ok = bits >> (4 * h);
+        f32x16 s = {};
+#pragma unroll
+        for (int x = 0; x < KS; ++x) s = mma(rk[x].frag(), qf[x], s);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * 64 + lane, row = c / (DP / 8);
+            tv.put(row, c - row * (DP / 8), rv[i].frag());
+        }
+        __builtin_amdgcn_wave_barrier();                          // (LDS accesses of one wave are in order)
+        j += 128;
+        settle();
+        if (j < end) fetch();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (!((ok >> acc_row(i, 0)) & 1)) s[i] = -INFINITY;
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(other_half_max(mx) * a.c, m);
+        const float sub = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - sub);
+        m = mx;
+        float lt = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -sub));
+            lt += s[i];
+        }
+        l = fmaf(l, f, lt);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        accumulate<NP>(o, tv, 0, s, lane);
+        __builtin_amdgcn_wave_barrier();
+    }
+    l = other_half_sum(l);
+    __syncthreads();                                              // the value tiles are read: their memory takes the partial outputs
+    float *out = (float *)mem;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *(f32x4 *)&out[(wave * 32 + col) * LO + 32 * t + 8 * i + 4 * h] = f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+    if (h == 0) {
+        wave_m[wave][col] = m;
+        wave_l[wave][col] = l;
+    }
+    __syncthreads();
+    const int r = threadIdx.x >> 3;                               // eight lanes per row
+    if (r >= a.R) return;
+    float f[4], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+        if (wave_l[w][r] != 0.0f) top = fmaxf(top, wave_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = wave_l[w][r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][r] - top);
+        sum = fmaf(wave_l[w][r], f[w], sum);
+    }
+    const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
+    const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+        const int d = 32 * t + 4 * (threadIdx.x & 7);
+        f32x4 x = {};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (f[w] != 0.0f) x[i] = fmaf(out[(w * 32 + r) * LO + d + i], f[w], x[i]);
+        if (a.splits > 1) store4(a.part + y * a.D, d, a.D, (a.D & 3) == 0, x[0], x[1], x[2], x[3]);
+        else store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, WIDE || (a.D & 7) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    }
+    if ((threadIdx.x & 7) == 0) {
+        if (a.splits > 1) {
+            a.part2[2 * y] = top;
+            a.part2[2 * y + 1] = sum;
+        } else if (a.lse) {
+            a.lse[(int64_t)bh * a.R + r] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------- backward
 // P is recomputed from the stored log2 of the softmax sum; delta = do . o is what the softmax subtracts from dP:
 //     dS = P (dP - delta),  dP = do V^T,  dq = scale dS K,  dk = scale dS^T q,  dv = P^T do
@@ -812,7 +965,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     const bool quad = (a.D & 3) == 0;
     const int64_t step = (MODE == 2 ? 2 : 1) * rows * a.D;
     const float *src = a.part + (which * rows + w) * a.D + d;
-#pragma unroll 4
+#pragma unroll 8
     for (int p0 = 0; p0 < a.splits; p0 += groups) {
         const int p = p0 + pg;
         const float wt = MODE == 0 ? __shfl(f, p & 63, 64) : 1.0f;
@@ -842,15 +995,17 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
 }
 
 // ------------------------------------------------------------------------------------------------- host side
-constexpr int kWant = 512;         // workgroups that fill the chip (two per CU)
 
-// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: none if those fill the chip, otherwise
-// enough to, with at least four tiles each, at most 64
-void split_of(int64_t blocks, int red, int &splits, int &per)
+// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: one if those give every CU one,
+// otherwise as many as make `want` workgroups, with at least `least` tiles each, at most 64.  (Above one workgroup per CU the
+// parts' round trip through memory costs more than the evener load gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in
+// one part, 338 in two.)
+constexpr int kCUs = 256;
+void split_of(int64_t blocks, int red, int64_t want, int least, int &splits, int &per)
 {
-    int64_t s = blocks > 0 && blocks < kWant / 2 ? kWant / blocks : 1;
+    int64_t s = blocks > 0 && blocks < kCUs ? want / blocks : 1;
     if (s > 64) s = 64;
-    if (s > red / 4) s = red / 4;
+    if (s > red / least) s = red / least;
     if (s < 1) s = 1;
     per = (int)((red + s - 1) / s);
     if (per < 1) per = 1;
@@ -881,7 +1036,8 @@ struct Plan {
     bool wide;                               // 16-byte loads
     int NP, DP, BK, BQ;
     int rtiles, ktiles;                      // workgroups along the rows, along the states
-    int fs, fper, ks, kper;                  // parts of the reduction and tiles of a part: over the states (forward, dq), over the rows
+    bool few;                                // forward: at most 32 rows, the waves divide the states
+    int fs, fper, qs, qper, ks, kper;        // parts of the reduction and tiles of a part: forward, dq (over the states), dkv (over the rows)
 };
 Plan plan_of(const mvf_attn_desc &d)
 {
@@ -895,8 +1051,11 @@ Plan plan_of(const mvf_attn_desc &d)
     const int64_t bh = (int64_t)d.B * d.Hk;
     p.rtiles = (R + 127) / 128;
     p.ktiles = (d.Lk + 127) / 128;
-    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, p.fs, p.fper);
-    split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, p.ks, p.kper);
+    p.few = R <= 32;
+    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, 2 * kCUs, 4, p.qs, p.qper);
+    if (p.few) split_of(bh, (d.Lk + 127) / 128, kCUs, 2, p.fs, p.fper);          // (one per CU: 59 us; two: 74 -- 5 x 40,001 x 80 fp32)
+    else p.fs = p.qs, p.fper = p.qper;
+    split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, 2 * kCUs, 4, p.ks, p.kper);
     return p;
 }
 bool bad_desc(const mvf_attn_desc *d)
@@ -931,6 +1090,12 @@ void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
     constexpr int BT = tile_states(NP, DP);
     if (a.wide) hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
     else hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+}
+template <int NP, int DP>
+void launch_few(const AttnArgs &a, int64_t blocks, hipStream_t st)
+{
+    if (a.wide) hipLaunchKernelGGL((k_attn_few<NP, DP, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_few<NP, DP, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
 void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
@@ -1000,7 +1165,8 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
-    MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
+    if (p.few) MVF_ATTN_PICK(launch_few, p, a, (int64_t)d->B * d->Hk * p.fs, st);
+    else MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
     if (p.fs > 1) launch_join<0>(a, p.NP, rows, st);
     return hip_check_launch();
 }
@@ -1011,7 +1177,7 @@ size_t mvf_cross_attention_bwd_workspace_bytes(const mvf_attn_desc *d)
     const Plan p = plan_of(*d);
     const int64_t rows = (int64_t)d->B * d->Hq * d->Lq, states = (int64_t)d->B * d->Hk * d->Lk;
     const int64_t delta = (rows + 3) / 4 * 4;
-    const int64_t pq = p.fs > 1 ? p.fs * rows * d->D : 0, pk = p.ks > 1 ? 2 * p.ks * states * d->D : 0;
+    const int64_t pq = p.qs > 1 ? p.qs * rows * d->D : 0, pk = p.ks > 1 ? 2 * p.ks * states * d->D : 0;
     return (size_t)((delta + (pq > pk ? pq : pk)) * 4);
 }
 
@@ -1034,9 +1200,9 @@ int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_BWD, st, tensor_bytes(*d, 4 * rows + 4 * states));
     if (d->Lq > 0) {
-        a.tiles = p.rtiles; a.splits = p.fs; a.per = p.fper;
-        MVF_ATTN_PICK(launch_dq, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
-        if (p.fs > 1) launch_join<1>(a, p.NP, rows, st);
+        a.tiles = p.rtiles; a.splits = p.qs; a.per = p.qper;
+        MVF_ATTN_PICK(launch_dq, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.qs, st);
+        if (p.qs > 1) launch_join<1>(a, p.NP, rows, st);
     }
     if (d->Lk > 0 && g_k) {
         a.tiles = p.ktiles; a.splits = p.ks; a.per = p.kper;
