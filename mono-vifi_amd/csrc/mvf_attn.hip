@@ -64,9 +64,8 @@ MVF_DEV float trunc_bf16(float x) { return __uint_as_float(__float_as_uint(x) & 
 MVF_DEV short top16(float x) { return (short)(__float_as_uint(x) >> 16); }
 
 // eight fp32 values -> NP planes of bf16.  One plane rounds to nearest even (half a step, 2^-8 of the value); three planes
-// cut, so that every remainder is exact.  (An infinity stays in plane 0 and leaves no remainder: what it multiplies becomes
-// infinite, or NaN where the other factor has an empty plane.  Probabilities and dS need no such care: INF false.)
-template <int NP, bool INF = true>
+// cut, so that every remainder is exact.  (An infinity leaves a NaN behind: what it takes part in becomes NaN.)
+template <int NP>
 MVF_DEV Frag<NP> split8(const float (&x)[8])
 {
     Frag<NP> f;
@@ -78,7 +77,7 @@ MVF_DEV Frag<NP> split8(const float (&x)[8])
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float hi = trunc_bf16(x[e]);
-            const float r1 = INF && __builtin_isinf(hi) ? 0.0f : x[e] - hi;
+            const float r1 = x[e] - hi;
             const float mid = trunc_bf16(r1);
             a[e] = top16(hi);
             b[e] = top16(mid);
@@ -114,6 +113,7 @@ struct Raw<1> {
     MVF_DEV void zero() { x = bf16x8{}; }
     MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at) { x = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0)); }
     MVF_DEV Frag<1> frag() const { return Frag<1>{{x}}; }
+    MVF_DEV Frag<1> frag_scaled(float) const { return frag(); }
 };
 template <>
 struct Raw<3> {
@@ -129,7 +129,16 @@ struct Raw<3> {
         const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
         return split8<3>(x);
     }
+    MVF_DEV Frag<3> frag_scaled(float f) const
+    {
+        const float x[8] = {a[0] * f, a[1] * f, a[2] * f, a[3] * f, b[0] * f, b[1] * f, b[2] * f, b[3] * f};
+        return split8<3>(x);
+    }
 };
+// The factor c of the exponent: three planes take it into q (or k) before it is cut, one rounding of fp32 among those of the
+// products, so that the scores come out of the matrix units ready; one plane would round the product to bf16.
+template <int NP>
+MVF_DEV float exponent(float s, float c, float minus) { return NP == 3 ? s + minus : fmaf(s, c, minus); }
 // channels d0 .. d0 + 7 of a row of D channels (zeros behind D, or if the row is not `live`); `wide`: rows are 16-byte aligned
 // and D is a multiple of 8
 MVF_DEV Raw<1> load8(const __bf16 *row, int d0, int D, bool wide, bool live)
@@ -281,29 +290,34 @@ struct Flight {
     typedef typename Elem<NP>::T T;
     static constexpr int CPR = DP / 8, CHUNKS = ROWS * CPR, N = (CHUNKS + NT - 1) / NT;
     Raw<NP> r[N];
+    static MVF_DEV int row_of(int i) { return (i * NT + (int)threadIdx.x) / CPR; }
+    static MVF_DEV int chan_of(int i) { return ((i * NT + (int)threadIdx.x) % CPR) * 8; }
+    // `all`: every row is valid (the same in every lane)
     template <typename V, typename F>
-    MVF_DEV void fetch(const T *base, int D, V valid, F off)
+    MVF_DEV void fetch(const T *base, int D, bool all, V valid, F off)
     {
-        __amdgpu_buffer_rsrc_t rs;
-        if constexpr (WIDE) rs = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, 0x7fffffff, 0x00027000);
+        if constexpr (WIDE) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(base), (short)0, 0x7fffffff, 0x00027000);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * NT + threadIdx.x, row = c / CPR, ch = c - row * CPR;
-            const bool in = (CHUNKS % NT == 0 || c < CHUNKS) && valid(row);
-            if constexpr (WIDE) {
-                r[i].load(rs, in && ch * 8 < D ? (uint32_t)(off(row) + ch * 8) * (uint32_t)sizeof(T) : kNowhere);
-            } else {
-                r[i] = load8(base + (in ? off(row) : 0), ch * 8, D, false, in);
+            for (int i = 0; i < N; ++i) {
+                const bool in = (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) && chan_of(i) < D;
+                uint32_t at = in ? (uint32_t)(off(i, row_of(i)) + chan_of(i)) * (uint32_t)sizeof(T) : kNowhere;
+                if (!all && !valid(row_of(i))) at = kNowhere;
+                r[i].load(rs, at);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool in = (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) && valid(row_of(i));
+                r[i] = load8(base + (in ? off(i, row_of(i)) : 0), chan_of(i), D, false, in);
             }
         }
     }
     MVF_DEV void commit(Tile<NP, ROWS, DP> &t) const
     {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = i * NT + threadIdx.x, row = c / CPR, ch = c - row * CPR;
-            if (CHUNKS % NT == 0 || c < CHUNKS) t.put(row, ch, r[i].frag());
-        }
+        for (int i = 0; i < N; ++i)
+            if (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) t.put(row_of(i), chan_of(i) / 8, r[i].frag());
     }
 };
 template <bool WIDE>
@@ -388,7 +402,7 @@ MVF_DEV Frag<NP> acc_frag(const f32x16 &x, int s)
     float y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
-    return split8<NP, false>(y);
+    return split8<NP>(y);
 }
 
 // four consecutive channels d .. d + 3 of a row
@@ -458,7 +472,7 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
     constexpr int KS = DP / 16, DT = DP / 32, KT = BK / 32;
-    constexpr float kSlack = 8.0f;            // the reference of the exponentials follows the maximum once it is 2^8 behind
+    constexpr float kMost = 1024.0f;
     __shared__ __attribute__((aligned(16))) Tile<NP, BK, DP> tile_k[buffers(NP)], tile_v[buffers(NP)];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
     int id = xcd_run(blockIdx.x, gridDim.x);
@@ -471,22 +485,33 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
     Walk<BK> w(a, b, part, lane);
     Flight<NP, BK, DP, WIDE> fk, fv;
-    const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
+    typedef typename Stride<WIDE>::T Off;
+    Off ok[fk.N], ov[fv.N];                                       // rows within a tile
+#pragma unroll
+    for (int i = 0; i < fk.N; ++i) {
+        ok[i] = fk.row_of(i) * (Off)a.ks[1];
+        ov[i] = fk.row_of(i) * (Off)a.vs[1];
+    }
     auto fetch = [&] {
         auto valid = [&](int row) { return ((uint32_t)(row & 32 ? w.bits >> 32 : w.bits) >> (row & 31)) & 1; };
-        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, valid, [&](int row) { return row * ks; });
-        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, valid, [&](int row) { return row * vs; });
+        const bool all = w.bits == Walk<BK>::kFull;
+        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, all, valid, [&](int i, int) { return ok[i]; });
+        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, all, valid, [&](int i, int) { return ov[i]; });
     };
     if (w.live()) fetch();
     Frag<NP> qf[KS];
     const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, r, hk, a.G) : 0);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+    for (int s = 0; s < KS; ++s) qf[s] = load8(qrow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
     f32x16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x16{};
-    float m = -INFINITY, sub = 0.0f, l = 0.0f;                    // reference and sum of the exponentials; sub: 0 while there is none
+    // reference and sum of the exponentials; sub: the reference, 0 while there is none.  The reference is the maximum of the
+    // first tile, and is looked at again only when a sum of exponentials outgrows it (kMost: far from the range of fp32, and
+    // bf16 keeps its relative precision): a maximum over every tile would be a sixth of the vector instructions.
+    float m = -INFINITY, sub = 0.0f, l = 0.0f;
     constexpr bool kTwo = buffers(NP) == 2;
+    bool first = true;
     int buf = 0;
     auto commit = [&] {
         fk.commit(tile_k[buf]);
@@ -504,27 +529,47 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
         w.next(a);
         if (w.live()) fetch();
         f32x16 s[KT];
+        auto scores = [&] {
 #pragma unroll
-        for (int t = 0; t < KT; ++t) s[t] = f32x16{};
-        stream<NP, KT * KS>([&](int i) { return tk.rows(32 * (i % KT), 16 * (i / KT), lane); },
-                            [&](int i, const Frag<NP> &f) { s[i % KT] = mma(f, qf[i / KT], s[i % KT]); });
-        if (bits != Walk<BK>::kFull) {
+            for (int t = 0; t < KT; ++t) s[t] = f32x16{};
+            stream<NP, KT * KS>([&](int i) { return tk.rows(32 * (i % KT), 16 * (i / KT), lane); },
+                                [&](int i, const Frag<NP> &f) { s[i % KT] = mma(f, qf[i / KT], s[i % KT]); });
+            if (bits != Walk<BK>::kFull) {
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+                for (int t = 0; t < KT; ++t) {
+                    const uint32_t in = (uint32_t)(bits >> (32 * t)) >> (4 * h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!((ok >> acc_row(i, 0)) & 1)) s[t][i] = -INFINITY;
+                    for (int i = 0; i < 16; ++i)
+                        if (!((in >> acc_row(i, 0)) & 1)) s[t][i] = -INFINITY;
+                }
             }
+        };
+        auto exps = [&] {
+            float lt = 0.0f;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[t][i] = __builtin_amdgcn_exp2f(exponent<NP>(s[t][i], a.c, -sub));
+                    lt += s[t][i];
+                }
+            return lt;
+        };
+        scores();
+        float lt = 0.0f;
+        bool again = first;
+        if (!first) {
+            lt = exps();
+            again = __any(lt > kMost || m == -INFINITY);
+            if (again) scores();
         }
-        float mx = s[0][0];
+        if (again) {
+            float mx = s[0][0];
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = other_half_max(mx) * a.c;
-        if (__any(mx > m + kSlack)) {
-            mx = fmaxf(mx, m);
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+            mx = fmaxf(other_half_max(mx) * (NP == 3 ? 1.0f : a.c), m);
             sub = mx == -INFINITY ? 0.0f : mx;
             const float f = __builtin_amdgcn_exp2f(m - sub);
             m = mx;
@@ -533,15 +578,9 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
+            lt = exps();
         }
-        float lt = 0.0f;
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], a.c, -sub));
-                lt += s[t][i];
-            }
+        first = false;
         l += lt;
 #pragma unroll
         for (int t = 0; t < KT; ++t) accumulate<NP>(o, tv, 32 * t, s[t], lane);
@@ -629,7 +668,7 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
     const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, col, hk, a.G) : 0);
     Frag<NP> qf[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+    for (int s = 0; s < KS; ++s) qf[s] = load8(qrow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
     f32x16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = f32x16{};
@@ -654,13 +693,13 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(other_half_max(mx) * a.c, m);
+        mx = fmaxf(other_half_max(mx) * (NP == 3 ? 1.0f : a.c), m);
         const float sub = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - sub);
         m = mx;
         float lt = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -sub));
+            s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, -sub));
             lt += s[i];
         }
         l = fmaf(l, f, lt);
@@ -725,6 +764,10 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
 // Two passes without atomics, so that the sums have one order: rows own dq (and write delta), states own dk and dv.  The
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
+// dP - delta: the products of dP start from -delta where sixteen registers more do not cost a wave per SIMD (1,280 x 2,560 x 128
+// bf16 backward: 311 -> 343 us)
+constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
+
 // grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
@@ -743,11 +786,18 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
     Walk<BK> w(a, b, part, lane);
     Flight<NP, BK, DP, WIDE> fk, fv;
-    const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
+    typedef typename Stride<WIDE>::T Off;
+    Off ok[fk.N], ov[fv.N];                                       // rows within a tile
+#pragma unroll
+    for (int i = 0; i < fk.N; ++i) {
+        ok[i] = fk.row_of(i) * (Off)a.ks[1];
+        ov[i] = fk.row_of(i) * (Off)a.vs[1];
+    }
     auto fetch = [&] {
         auto valid = [&](int row) { return ((uint32_t)(row & 32 ? w.bits >> 32 : w.bits) >> (row & 31)) & 1; };
-        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, valid, [&](int row) { return row * ks; });
-        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, valid, [&](int row) { return row * vs; });
+        const bool all = w.bits == Walk<BK>::kFull;
+        fk.fetch(kb + (int64_t)w.j * a.ks[1], a.D, all, valid, [&](int i, int) { return ok[i]; });
+        fv.fetch(vb + (int64_t)w.j * a.vs[1], a.D, all, valid, [&](int i, int) { return ov[i]; });
     };
     if (w.live()) fetch();
     Frag<NP> qf[KS], gf[KS];
@@ -756,7 +806,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     float delta = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        qf[s] = load_frag<NP>(qrow, 16 * s + 8 * h, a.D, WIDE, live);
+        qf[s] = load8(qrow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
         const Raw<NP> g = load8((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
         delta = dot8(g, load8((const T *)a.o + dense, 16 * s + 8 * h, a.D, dwide, live), delta);
         gf[s] = g.frag();
@@ -764,9 +814,11 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     delta = other_half_sum(delta);
     const float lse = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
     if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta;
-    f32x16 dq[DT];
+    f32x16 dq[DT], minus_delta;
 #pragma unroll
     for (int t = 0; t < DT; ++t) dq[t] = f32x16{};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) minus_delta[i] = -delta;
     constexpr bool kTwo = buffers(NP) == 2;
     int buf = 0;
     auto commit = [&] {
@@ -787,6 +839,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             f32x16 s = {}, dp = {};
+            if (start_at_delta(NP, DP)) dp = minus_delta;
             stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tv : tk).rows(32 * t, 16 * (i / 2), lane); },
                                [&](int i, const Frag<NP> &f) {
                                    if (i % 2) dp = mma(f, gf[i / 2], dp);
@@ -795,13 +848,14 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
             // a state that does not count: its row of the tile is zero, so whatever dS holds for it adds nothing to dq --
             // but exp2(-lse) may be infinite there, so it is cleared
             if (bits != Walk<BK>::kFull) {
-                const uint32_t ok = (uint32_t)(bits >> (32 * t)) >> (4 * h);
+                const uint32_t in = (uint32_t)(bits >> (32 * t)) >> (4 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (!((ok >> acc_row(i, 0)) & 1)) s[i] = -INFINITY;
+                    if (!((in >> acc_row(i, 0)) & 1)) s[i] = -INFINITY;
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.c, -lse)) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i)
+                s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, -lse)) * (start_at_delta(NP, DP) ? dp[i] : dp[i] - delta);
             accumulate<NP>(dq, tk, 32 * t, s, lane);
         }
         if (kTwo) {
@@ -838,7 +892,8 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     int r0 = part * a.per * BQ;
     Flight<NP, BQ, DP, WIDE> fq, fg;
     float pl = 0.0f, pd = 0.0f;
-    const typename Stride<WIDE>::T qs1 = a.qs[1], qs2 = a.qs[2], gs1 = (int64_t)a.Hq * a.D, gs2 = a.D;
+    typedef typename Stride<WIDE>::T Off;
+    const Off qs1 = a.qs[1], qs2 = a.qs[2], gs1 = (int64_t)a.Hq * a.D, gs2 = a.D;
     const float invG = 1.0f / (float)a.G;
     auto fetch = [&] {
         // row r0 + row is token i0 + i, head g of the group: (g0 + row) / G by a product, exact for the small numbers that come up
@@ -848,12 +903,13 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
         auto token = [&](int row) { return (int)(((float)(g0 + row) + 0.5f) * invG); };
         const T *qb = (const T *)a.q + (int64_t)b * a.qs[0] + (int64_t)hk * a.G * a.qs[2] + (int64_t)i0 * a.qs[1];
         const T *gb = (const T *)a.go + (((int64_t)b * a.Lq + i0) * a.Hq + (int64_t)hk * a.G) * a.D;
-        fq.fetch(qb, a.D, valid, [&](int row) { const int i = token(row); return i * qs1 + (g0 + row - i * a.G) * qs2; });
-        fg.fetch(gb, a.D, valid, [&](int row) { const int i = token(row); return i * gs1 + (g0 + row - i * a.G) * gs2; });
+        const bool all = r0 + BQ <= a.R;
+        fq.fetch(qb, a.D, all, valid, [&](int, int row) { const int i = token(row); return i * qs1 + (g0 + row - i * a.G) * qs2; });
+        fg.fetch(gb, a.D, all, valid, [&](int, int row) { const int i = token(row); return i * gs1 + (g0 + row - i * a.G) * gs2; });
         if (threadIdx.x < BQ) {
             const int r = r0 + threadIdx.x;
-            pl = r < a.R ? a.lse[(int64_t)bh * a.R + r] : INFINITY;            // rows behind the last: P = 0
-            pd = r < a.R ? a.delta[(int64_t)bh * a.R + r] : 0.0f;
+            pl = r < a.R ? -a.lse[(int64_t)bh * a.R + r] : -INFINITY;          // rows behind the last: P = 0
+            pd = r < a.R ? -a.delta[(int64_t)bh * a.R + r] : 0.0f;
         }
     };
     constexpr bool kTwo = buffers(NP) == 2;
@@ -873,7 +929,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     Frag<NP> kf[KS], vf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        kf[s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, WIDE, live);
+        kf[s] = load8(krow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
         vf[s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, WIDE, live);
     }
     f32x16 dk[DT], dv[DT];
@@ -892,22 +948,26 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
         if (r0 < r1) fetch();
 #pragma unroll
         for (int u = 0; u < QT; ++u) {
+            constexpr bool kStart = start_at_delta(NP, DP);
             f32x16 s = {}, dp = {};
+            auto row4 = [&](const float *x, int i) { return *(const f32x4 *)&x[32 * u + acc_row(4 * i, h)]; };     // of elements 4 i ..
+            if (kStart) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    dp[i] = row4(sd, i / 4)[i % 4];
+                    if (NP == 3) s[i] = row4(sl, i / 4)[i % 4];  // (the exponents start from -lse likewise)
+                }
+            }
             stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tg : tq).rows(32 * u, 16 * (i / 2), lane); },
                                [&](int i, const Frag<NP> &f) {
                                    if (i % 2) dp = mma(f, vf[i / 2], dp);
                                    else s = mma(f, kf[i / 2], s);
                                });
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 ls = *(const f32x4 *)&sl[32 * u + acc_row(4 * i, h)], de = *(const f32x4 *)&sd[32 * u + acc_row(4 * i, h)];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // (the column of a state that does not count is dropped at the end)
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * i + e], a.c, -ls[e]));
-                    s[4 * i + e] = p;
-                    dp[4 * i + e] = p * (dp[4 * i + e] - de[e]);
-                }
+            for (int i = 0; i < 16; ++i) {
+                // (the column of a state that does not count is dropped at the end)
+                s[i] = __builtin_amdgcn_exp2f(NP == 3 ? s[i] : fmaf(s[i], a.c, row4(sl, i / 4)[i % 4]));
+                dp[i] = s[i] * (kStart ? dp[i] : dp[i] + row4(sd, i / 4)[i % 4]);
             }
             accumulate<NP>(dv, tg, 32 * u, s, lane);
             accumulate<NP>(dk, tq, 32 * u, dp, lane);
@@ -996,14 +1056,14 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
 
 // ------------------------------------------------------------------------------------------------- host side
 
-// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: one if those give every CU one,
-// otherwise as many as make `want` workgroups, with at least `least` tiles each, at most 64.  (Above one workgroup per CU the
-// parts' round trip through memory costs more than the evener load gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in
-// one part, 338 in two.)
+// parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: as many as fit one workgroup per CU,
+// with at least `least` tiles each, at most 64.  (More cost more in the parts' round trip through memory than the evener load
+// gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in one part, 338 in two; 192 of 480 x 960 x 32 backward: 65 and 73;
+// 72 of 333 x 1,281 x 28 fp32: 69, 46, 36, 38 us in 1, 2, 3, 5; 5 x 40,001 x 80 fp32: 59 us at 252 workgroups, 74 at 384.)
 constexpr int kCUs = 256;
-void split_of(int64_t blocks, int red, int64_t want, int least, int &splits, int &per)
+void split_of(int64_t blocks, int red, int least, int &splits, int &per)
 {
-    int64_t s = blocks > 0 && blocks < kCUs ? want / blocks : 1;
+    int64_t s = blocks > 0 ? kCUs / blocks : 1;
     if (s > 64) s = 64;
     if (s > red / least) s = red / least;
     if (s < 1) s = 1;
@@ -1052,10 +1112,10 @@ Plan plan_of(const mvf_attn_desc &d)
     p.rtiles = (R + 127) / 128;
     p.ktiles = (d.Lk + 127) / 128;
     p.few = R <= 32;
-    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, 2 * kCUs, 4, p.qs, p.qper);
-    if (p.few) split_of(bh, (d.Lk + 127) / 128, kCUs, 2, p.fs, p.fper);          // (one per CU: 59 us; two: 74 -- 5 x 40,001 x 80 fp32)
+    split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, 4, p.qs, p.qper);
+    if (p.few) split_of(bh, (d.Lk + 127) / 128, 2, p.fs, p.fper);
     else p.fs = p.qs, p.fper = p.qper;
-    split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, 2 * kCUs, 4, p.ks, p.kper);
+    split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, 4, p.ks, p.kper);
     return p;
 }
 bool bad_desc(const mvf_attn_desc *d)
