@@ -9,10 +9,14 @@ import torch
 _CACHE = {}
 
 
-def const_tensor(values, device, dtype=torch.float32):
-    key = (tuple(float(v) for v in values), str(device), dtype)
+def cached(key, make):
+    """The tensor ``make()`` returned the first time ``key`` came up."""
     t = _CACHE.get(key)
     if t is None:
-        t = torch.tensor([float(v) for v in values], dtype=dtype, device=device)
-        _CACHE[key] = t
+        t = _CACHE[key] = make()
     return t
+
+
+def const_tensor(values, device, dtype=torch.float32):
+    return cached((tuple(float(v) for v in values), str(device), dtype),
+                  lambda: torch.tensor([float(v) for v in values], dtype=dtype, device=device))

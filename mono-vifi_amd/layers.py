@@ -10,6 +10,9 @@ module (reference: layers.py:16-311), so ``from layers import *`` call sites kee
 plus ``grid_sample_border_ac`` -- the exact ``F.grid_sample(..., padding_mode="border",
 align_corners=True)`` call of train.py:966-969 as a standalone op.
 
+and ``CrossAttention`` / ``token_positions``: attention between the tokens of frames, which the reference
+does not have (networks/fusion_module.py, ``--fusion_attention``).
+
 Hot-path functions execute as hand-written HIP kernels through the C ABI
 (include/mvf_hotpath.h); they require HIP tensors and have no CPU fallback.  The conv
 building blocks are plain ``torch.nn`` modules (MIOpen / hipBLASLt do the contractions).
@@ -22,7 +25,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import consts, ops
 
 
 # ----------------------------------------------------------------------------- geometry
@@ -253,6 +256,44 @@ class ConvBlock1x1(nn.Module):
 
     def forward(self, x):
         return conv_bias_act(self.conv.conv, x, "elu")
+
+
+# ----------------------------------------------------------------------------- token attention
+def token_positions(height, width, frames, device):
+    """int32 [frames * height * width, 3]: frame, row and column of the tokens of ``frames`` (their indices, e.g. (-1, 1)), row-major
+    within a frame.  Created once per argument set (``consts.const_tensor``): callers must not modify it."""
+    key = ("token_positions", height, width, tuple(frames), str(device))
+    pos = consts.cached(key, lambda: torch.stack(torch.meshgrid(
+        torch.tensor(list(frames)), torch.arange(height), torch.arange(width), indexing="ij"), -1).reshape(-1, 3).int().to(device))
+    return pos
+
+
+class CrossAttention(nn.Module):
+    """Multi-head attention of the tokens of one frame to the tokens of others; no counterpart in the reference.
+
+    ``x [B, Lq, dim]`` attends to ``states [B, Lk, states_dim]``: projections, RMS norm of every query and key head with the position
+    rotation (``ops.qk_norm_rope``; positions int32 ``[L, axes]``, or None for the norm alone), attention
+    (``ops.cross_attention``; ``num_kv_heads`` < ``num_heads`` shares states between query heads; ``key_mask`` / ``kv_lens`` say which
+    states count), output projection.  HIP device only, float32 or bfloat16 (also under autocast)."""
+
+    def __init__(self, dim, num_heads=8, num_kv_heads=None, states_dim=None, bias=True, base=100.0):
+        super().__init__()
+        num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        if dim % num_heads or num_heads % num_kv_heads:
+            raise ValueError(f"{dim} channels, {num_heads} heads and {num_kv_heads} heads of the states do not divide")
+        self.num_heads, self.num_kv_heads, self.head_dim, self.base = num_heads, num_kv_heads, dim // num_heads, float(base)
+        self.q = nn.Linear(dim, dim, bias=bias)
+        self.kv = nn.Linear(dim if states_dim is None else states_dim, 2 * num_kv_heads * self.head_dim, bias=bias)
+        self.q_norm = nn.Parameter(torch.ones(self.head_dim))
+        self.k_norm = nn.Parameter(torch.ones(self.head_dim))
+        self.proj = nn.Linear(dim, dim, bias=bias)
+
+    def forward(self, x, states, x_pos=None, states_pos=None, key_mask=None, kv_lens=None):
+        q = self.q(x).unflatten(-1, (self.num_heads, self.head_dim))
+        kv = self.kv(states).unflatten(-1, (2, self.num_kv_heads, self.head_dim))
+        q, k = ops.qk_norm_rope(q, kv[:, :, 0], self.q_norm, self.k_norm, x_pos, states_pos, base=self.base)
+        out = ops.cross_attention(q, k, kv[:, :, 1], key_mask=key_mask, kv_lens=kv_lens)
+        return self.proj(out.flatten(2))
 
 
 def compute_depth_errors(gt, pred):

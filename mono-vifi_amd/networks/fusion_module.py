@@ -3,12 +3,13 @@ sin/cos embedding of the flow, mask-merge and mix with a 1x1 conv per scale.
 
 API / state-dict keys follow reference networks/fusion_module.py (``Embedder`` 7-37,
 ``FusionModule`` 40-130; parameters under ``fusion_conv.<n>.conv.conv.*``, coarsest scale
-first)."""
+first).  ``--fusion_attention N`` (0 by default; not in the reference) lets the fused features of the N coarsest
+levels attend to the tokens of both neighbours as well (parameters under ``cross_frame.<n>``, coarsest first)."""
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..layers import ConvBlock1x1
+from ..layers import ConvBlock1x1, CrossAttention, token_positions
 from .ifrnet import warp
 from ..consts import const_tensor
 
@@ -33,6 +34,25 @@ class Embedder:
         return torch.cat(parts, 1)
 
 
+class CrossFrame(nn.Module):
+    """fused [B,C,H,W] + attention of the centre frame's tokens to those of the two neighbours; positions are (frame, row,
+    column).  The output projection starts at zero: at first the fused features pass unchanged."""
+
+    def __init__(self, channels):
+        super().__init__()
+        heads = next(h for h in range(8, 0, -1) if channels % h == 0 and channels // h >= 6)
+        self.attn = CrossAttention(channels, heads)
+        nn.init.zeros_(self.attn.proj.weight)
+        nn.init.zeros_(self.attn.proj.bias)
+
+    def forward(self, fused, centre, before, after):
+        B, C, H, W = centre.shape
+        x = centre.flatten(2).transpose(1, 2)
+        states = torch.stack([before, after], 1).flatten(3).transpose(2, 3).reshape(B, 2 * H * W, C)
+        y = self.attn(x, states, token_positions(H, W, (0,), x.device), token_positions(H, W, (-1, 1), x.device))
+        return fused + y.transpose(1, 2).reshape(B, C, H, W).to(fused.dtype)
+
+
 class FusionModule(nn.Module):
     def __init__(self, args, num_ch_enc, embed_multires=10):
         super().__init__()
@@ -45,6 +65,16 @@ class FusionModule(nn.Module):
         self.fusion_conv = nn.ModuleList([
             ConvBlock1x1(2 * (int(num_ch_enc[i]) + self.embedder_obj.out_dim), int(num_ch_enc[i]))
             for i in range(n - 1, -1, -1)])
+        self.attention_levels = min(n, int(getattr(args, "fusion_attention", 0)))
+        if self.attention_levels:
+            self.cross_frame = nn.ModuleList([CrossFrame(int(num_ch_enc[n - 1 - j])) for j in range(self.attention_levels)])
+
+    def _attend(self, fused, feats_0, feats_n1, feats_p1):
+        n = len(fused)
+        for j in range(self.attention_levels):
+            i = n - 1 - j
+            fused[i] = self.cross_frame[j](fused[i], feats_0[i], feats_n1[i], feats_p1[i])
+        return fused
 
     def get_embedding_flow(self, x):
         outs = []
@@ -72,10 +102,11 @@ class FusionModule(nn.Module):
             from .. import ops
             sizes = [tuple(f.shape[-2:]) for f in feats_0]
             preps = ops.fusion_prep(flow_0_n1, flow_0_p1, merge_mask, sizes, self.backbone == "LiteMono")
-            return [self.fusion_conv[self._slot[i]](
+            outs = [self.fusion_conv[self._slot[i]](
                 ops.fusion_level(feats_0[i].float(), feats_n1[i].float(), feats_p1[i].float(), preps[i],
                                  lists=(preps.lists, i)))
                 for i in range(len(feats_0))]
+            return self._attend(outs, feats_0, feats_n1, feats_p1)
         w_n1 = self.warp_features(feats_n1, flow_0_n1)
         w_p1 = self.warp_features(feats_p1, flow_0_p1)
         e_0 = self.get_embedding_flow(torch.zeros_like(flow_0_n1))
@@ -90,4 +121,4 @@ class FusionModule(nn.Module):
             m = F.interpolate(merge_mask, size=(H, W), mode="bilinear", align_corners=False)
             merged = m * fn + (1 - m) * fp
             outs.append(self.fusion_conv[self._slot[i]](torch.cat([f0, merged], 1)))
-        return outs
+        return self._attend(outs, feats_0, feats_n1, feats_p1)

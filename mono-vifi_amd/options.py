@@ -151,6 +151,9 @@ def build_parser():
                         "and the capturable AdamW (learning rate resident on the device).  backward: networks, "
                         "hot-path units, backward pass and gradient exchange; clipping and the ordinary optimiser "
                         "stay ~20 eager launches")
+    p.add_argument("--fusion_attention", type=int, default=0,
+                   help="number of pyramid levels, coarsest first, whose fused features also attend to the tokens of both "
+                        "neighbour frames (layers.CrossAttention); 0 = the reference's fusion")
     p.add_argument("--bucket_mb", type=float, default=32.0, help="gradient all-reduce bucket size")
     p.add_argument("--grad_exchange", type=str, default="all_reduce", choices=["all_reduce", "reduce_scatter"],
                    help="per gradient bucket: one RCCL all-reduce, or its two halves issued explicitly on "

@@ -549,6 +549,113 @@ def test_two_captured_graphs_replay():
                 assert torch.equal(a, b)
 
 
+# ------------------------------------------------------------------------------------------------ the modules that use them
+def layer_ref(m, x, states, xp, sp, allowed):
+    """layers.CrossAttention in 64 bits from its parameters."""
+    P = {n: p.detach().double().requires_grad_(True) for n, p in m.named_parameters()}
+    hd, H, Hk = m.head_dim, m.num_heads, m.num_kv_heads
+
+    def norm_rope(t, w, pos):
+        n = t * ((t * t).mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+        axes = pos.shape[-1]
+        ra = hd // (2 * axes) * 2
+        out = []
+        for a in range(axes):
+            lo, hi = n[..., a * ra:a * ra + ra // 2], n[..., a * ra + ra // 2:(a + 1) * ra]
+            ang = (pos[:, a, None].double() * m.base ** (-torch.arange(0, ra, 2, device=t.device, dtype=torch.float64) / ra))[:, None]
+            out += [lo * ang.cos() - hi * ang.sin(), lo * ang.sin() + hi * ang.cos()]
+        return torch.cat(out + [n[..., axes * ra:]], -1)
+    q = torch.nn.functional.linear(x, P["q.weight"], P["q.bias"]).unflatten(-1, (H, hd))
+    kv = torch.nn.functional.linear(states, P["kv.weight"], P["kv.bias"]).unflatten(-1, (2, Hk, hd))
+    q, k = norm_rope(q, P["q_norm"], xp), norm_rope(kv[:, :, 0], P["k_norm"], sp)
+    k, v = (t.repeat_interleave(H // Hk, 2).permute(0, 2, 1, 3) for t in (k, kv[:, :, 1]))
+    s = (q.permute(0, 2, 1, 3) @ k.transpose(-1, -2).contiguous() * hd ** -0.5).masked_fill(~allowed[:, None, None, :], -math.inf)
+    y = (torch.softmax(s, -1) @ v).permute(0, 2, 1, 3).flatten(2)
+    return torch.nn.functional.linear(y, P["proj.weight"], P["proj.bias"]), P
+
+
+@gpu
+@pytest.mark.parametrize("autocast", [False, True], ids=["f32", "autocast"])
+def test_the_layer(autocast):
+    """Projections, norm, rotation and attention of layers.CrossAttention with shared heads and a padded batch, against the formulas
+    in 64 bits: relative 2-norm, 8 roundings of the type in a row (3 projections, q / k, P, dS, output, gradient); for fp32, whose
+    products go through the library's matrix kernels, 1e-4."""
+    from mono_vifi_amd import layers
+    torch.manual_seed(0)
+    m = layers.CrossAttention(48, num_heads=4, num_kv_heads=2, states_dim=32).cuda()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, 30, 48, device="cuda", generator=g, requires_grad=True)
+    st = torch.randn(2, 60, 32, device="cuda", generator=g, requires_grad=True)
+    go = torch.randn(2, 30, 48, device="cuda", generator=g)
+    xp, sp = layers.token_positions(5, 6, (0,), x.device), layers.token_positions(5, 6, (-1, 1), x.device)
+    assert sp.shape == (60, 3) and sp[31].tolist() == [1, 0, 1] and layers.token_positions(5, 6, (-1, 1), x.device) is sp
+    lens = torch.tensor([60, 37], dtype=torch.int32, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+        y = m(x, st, xp, sp, kv_lens=lens)
+    assert y.dtype == (torch.bfloat16 if autocast else torch.float32)
+    names = [n for n, _ in m.named_parameters()]
+    got = [y] + list(torch.autograd.grad(y, [x, st] + [p for _, p in m.named_parameters()], go.to(y.dtype)))
+    xr, sr = x.detach().double().requires_grad_(True), st.detach().double().requires_grad_(True)
+    want, P = layer_ref(m, xr, sr, xp, sp, torch.arange(60, device="cuda") < lens[:, None])
+    wants = [want] + list(torch.autograd.grad(want, [xr, sr] + [P[n] for n in names], go.double()))
+    tol = 8 * 2.0 ** -8 if autocast else 1e-4
+    for n, a, b in zip(["y", "x", "states"] + names, got, wants):
+        assert float((a.double() - b).norm()) <= tol * float(b.norm()), n
+
+
+@gpu
+def test_fusion_module_attends(tmp_path):
+    """--fusion_attention: the same fused features at first (the output projection starts at zero), gradients in every parameter of
+    the attention once it does not, checkpoint keys beside the reference's."""
+    from types import SimpleNamespace
+    from mono_vifi_amd.networks import FusionModule
+    ch = [64, 64, 128, 256, 512]
+    torch.manual_seed(0)
+    plain = FusionModule(SimpleNamespace(backbone="ResNet18"), ch).cuda()
+    with_attn = FusionModule(SimpleNamespace(backbone="ResNet18", fusion_attention=2), ch).cuda()
+    extra = set(with_attn.state_dict()) - set(plain.state_dict())
+    assert all(k.startswith("cross_frame.") for k in extra) and len(extra) == 2 * 8
+    with_attn.load_state_dict(plain.state_dict(), strict=False)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    feats = [[r(2, c, 64 >> i, 96 >> i) for i, c in zip(range(1, 6), ch)] for _ in range(3)]
+    flows, mask = [3 * r(2, 2, 64, 96) for _ in range(2)], torch.rand(2, 1, 64, 96, device="cuda", generator=g)
+    a, b = plain(feats, flows, mask), with_attn(feats, flows, mask)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for m in with_attn.cross_frame:
+        torch.nn.init.normal_(m.attn.proj.weight, std=0.05)
+    out = with_attn(feats, flows, mask)
+    assert all(torch.equal(out[i], a[i]) for i in range(3)) and not torch.equal(out[4], a[4]) and not torch.equal(out[3], a[3])
+    sum(o.square().mean() for o in out).backward()
+    for n, p in with_attn.cross_frame.named_parameters():
+        assert torch.isfinite(p.grad).all() and float(p.grad.norm()) > 0, n
+
+
+@gpu
+@pytest.mark.parametrize("amp", [False, True], ids=["f32", "amp_bf16"])
+def test_training_step_with_fusion_attention(tmp_path, amp):
+    from test_trainer_gpu import device_batch, make_trainer
+    t = make_trainer(tmp_path, fusion_attention=2, amp_bf16=amp)
+    t.set_train()
+    proj = t.models["fusion_module"].cross_frame[0].attn.proj.weight
+    assert not proj.any()
+    batch = device_batch(2, 64, 96, t.device)
+    for _ in range(2):
+        losses = t.optimisation_step(dict(batch))
+        assert math.isfinite(float(losses["loss"]))
+    assert proj.any() and all(torch.isfinite(p).all() for p in t.models["fusion_module"].parameters())
+
+
+def test_the_layer_refuses_heads_that_do_not_divide():
+    from mono_vifi_amd import layers
+    for args in ((50, 8), (48, 4, 3)):
+        with pytest.raises(ValueError, match="do not divide"):
+            layers.CrossAttention(*args)
+    m = layers.CrossAttention(16, 2)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        m(torch.zeros(1, 3, 16), torch.zeros(1, 4, 16))
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def cpu(*shape, dtype=torch.float32):
     return torch.zeros(shape, dtype=dtype)
