@@ -254,6 +254,28 @@ def lib():
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The extension module with the token-attention autograd functions (csrc/mvf_torch.cpp), bound once to the entry points of
+    the loaded library."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.util
+        handle = lib()
+        path = os.path.join(_HERE, "lib", "_mvf_torch.so")
+        if not os.path.exists(path):
+            raise NativeLibraryError(f"{path} not found: run `python __graft_entry__.py` (or `make -C mono-vifi_amd/csrc`)")
+        spec = importlib.util.spec_from_file_location("_mvf_torch", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({n: C.cast(getattr(handle, n), C.c_void_p).value for n in EXPORTS
+                     if n.startswith(("mvf_cross_attention", "mvf_qk_norm", "mvf_error_string"))})
+        _torch_ops = module
+    return _torch_ops
+
+
 def check(err, what):
     if err != 0:
         msg = lib().mvf_error_string(err)

@@ -765,7 +765,8 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
 // dP - delta: the products of dP start from -delta where sixteen registers more do not cost a wave per SIMD (1,280 x 2,560 x 128
-// bf16 backward: 311 -> 343 us)
+// bf16 backward: 311 -> 343 us).  (The scores do not start from -lse: it outweighs their terms, and each sum would round at its
+// size -- dk and dv of 120 x 240 x 64 fp32: 4e-7 -> 1e-6 of the result.)
 constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
 
 // grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
@@ -953,10 +954,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
             auto row4 = [&](const float *x, int i) { return *(const f32x4 *)&x[32 * u + acc_row(4 * i, h)]; };     // of elements 4 i ..
             if (kStart) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    dp[i] = row4(sd, i / 4)[i % 4];
-                    if (NP == 3) s[i] = row4(sl, i / 4)[i % 4];  // (the exponents start from -lse likewise)
-                }
+                for (int i = 0; i < 16; ++i) dp[i] = row4(sd, i / 4)[i % 4];
             }
             stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tg : tq).rows(32 * u, 16 * (i / 2), lane); },
                                [&](int i, const Frag<NP> &f) {
@@ -966,7 +964,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 // (the column of a state that does not count is dropped at the end)
-                s[i] = __builtin_amdgcn_exp2f(NP == 3 ? s[i] : fmaf(s[i], a.c, row4(sl, i / 4)[i % 4]));
+                s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, row4(sl, i / 4)[i % 4]));
                 dp[i] = s[i] * (kStart ? dp[i] : dp[i] + row4(sd, i / 4)[i % 4]);
             }
             accumulate<NP>(dv, tg, 32 * u, s, lane);

@@ -9,8 +9,6 @@ surrounding MIOpen kernels and with DDP's reducer through normal stream semantic
 from __future__ import annotations
 
 import ctypes as C
-import functools
-import math
 
 import numpy as np
 import torch
@@ -1883,217 +1881,27 @@ def color_jitter(img, factors, order, apply, flip, frames=1, want_raw=False):
 
 
 # ------------------------------------------------------------------ token attention
-_ATTN_TYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16}
-
-
-def _token_heads(what, name, t, dtype=None):
-    """[batch, token, head, channel] with adjacent channels, float32 or bfloat16; any strides otherwise."""
-    if not torch.is_tensor(t) or t.dim() != 4:
-        raise RuntimeError(f"{what}: {name} must be [batch, tokens, heads, channels], got "
-                           f"{tuple(t.shape) if torch.is_tensor(t) else type(t).__name__}")
-    if t.dtype is not dtype:
-        if t.dtype not in _ATTN_TYPES:
-            raise RuntimeError(f"{what}: {name} must be float32 or bfloat16, got {t.dtype}")
-        if dtype is not None:
-            raise RuntimeError(f"{what}: {name} is {t.dtype}, the queries are {dtype}")
-    _, _, H, D = t.shape
-    if H < 1 or not 1 <= D <= nat.ATTN_MAX_D:
-        raise RuntimeError(f"{what}: {name} needs at least one head of 1..{nat.ATTN_MAX_D} channels, got {tuple(t.shape)}")
-    return t if D == 1 or t.stride(3) == 1 else t.contiguous()
-
-
-def _once(what):
-    # (torch's once_differentiable looks at the incoming gradient alone: a second derivative through the saved inputs would
-    # be silently missing)
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{what} is differentiable once: its backward does not run under create_graph=True")
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _aligned(g, dtype):
-    """An incoming gradient as the kernels read it: contiguous, of the forward's type, 16-byte aligned."""
-    if g.dtype is not dtype:
-        g = g.to(dtype)
-    g = g.contiguous()
-    return g.clone() if g.data_ptr() & 15 else g
-
-
-def _attn_desc(q, k, v, key_mask, kv_lens, scale):
-    B, Lq, Hq, D = q.shape
-    d = nat.AttnDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), B=B, Lq=Lq, Lk=k.shape[1], Hq=Hq, Hk=k.shape[2], D=D,
-                     dtype=_ATTN_TYPES[q.dtype], scale=scale)
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    if kv_lens is not None:
-        d.kv_lens = kv_lens.data_ptr()
-    if key_mask is not None:
-        d.key_mask = key_mask.data_ptr()
-        d.mask_stride[:] = key_mask.stride()
-    return d
-
-
-def _attn_forward(q, k, v, key_mask, kv_lens, scale, with_lse):
-    lib = nat.lib()
-    d = _attn_desc(q, k, v, key_mask, kv_lens, scale)
-    ref = C.byref(d)
-    dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if with_lse else None
-    n = lib.mvf_cross_attention_fwd_workspace_bytes(ref)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    nat.check(lib.mvf_cross_attention_fwd(ref, out.data_ptr(), _addr(lse), _addr(ws), _raw_stream()), "cross_attention_fwd")
-    return out, lse, d
-
-
-class CrossAttention(torch.autograd.Function):
-    """softmax(scale q k^T) v over the states that count (csrc/mvf_attn.hip).  No counterpart in the reference, whose fusion of
-    neighbour frames is a warp and a mask (networks/fusion_module.py:100-130)."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, key_mask, kv_lens, scale):
-        out, lse, d = _attn_forward(q, k, v, key_mask, kv_lens, scale, True)
-        ctx.save_for_backward(q, k, v, key_mask, kv_lens, out, lse)
-        ctx.scale, ctx.desc = scale, d
-        return out
-
-    @staticmethod
-    def backward(ctx, g):
-        _once("cross_attention")
-        q, k, v, key_mask, kv_lens, out, lse = ctx.saved_tensors
-        lib, d, dev = nat.lib(), ctx.desc, q.device
-        if d.q != q.data_ptr() or d.k != k.data_ptr() or d.v != v.data_ptr() or d.key_mask != _addr(key_mask) or d.kv_lens != _addr(kv_lens):
-            d = _attn_desc(q, k, v, key_mask, kv_lens, ctx.scale)       # saved tensors that were packed and came back elsewhere
-        ref = C.byref(d)
-        g, out, lse = _aligned(g, q.dtype), _aligned(out, q.dtype), lse.contiguous()
-        need = ctx.needs_input_grad
-        gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        gk = gv = None
-        if need[1] or need[2]:
-            gk, gv = torch.empty(k.shape, dtype=q.dtype, device=dev), torch.empty(v.shape, dtype=q.dtype, device=dev)
-        ws = torch.empty(lib.mvf_cross_attention_bwd_workspace_bytes(ref), dtype=torch.uint8, device=dev)
-        nat.check(lib.mvf_cross_attention_bwd(ref, out.data_ptr(), lse.data_ptr(), g.data_ptr(), gq.data_ptr(), _addr(gk), _addr(gv),
-                                              ws.data_ptr(), _raw_stream()), "cross_attention_bwd")
-        return gq if need[0] else None, gk if need[1] else None, gv if need[2] else None, None, None, None
-
-
+# (the autograd functions are csrc/mvf_torch.cpp: at the sizes of a coarse pyramid level the host decides, and a Function
+# written in Python doubles the time of a training call)
 def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
-    """Attention of the queries ``q [B, Lq, Hq, D]`` to the states ``k, v [B, Lk, Hk, D]`` of another length -> ``[B, Lq, Hq, D]``.
+    """Attention of the queries ``q [B, Lq, Hq, D]`` to the states ``k, v [B, Lk, Hk, D]`` of another length -> ``[B, Lq, Hq, D]``
+    (csrc/mvf_attn.hip).  No counterpart in the reference, whose fusion of neighbour frames is a warp and a mask
+    (networks/fusion_module.py:100-130).
 
     ``Hq`` is a multiple of ``Hk``: query head h reads head ``h // (Hq // Hk)`` of the states.  float32 or bfloat16, at most 128
     channels per head, any strides (channels adjacent; otherwise copied).  ``scale`` (> 0, default ``1 / sqrt(D)``) multiplies
     the scores.  ``kv_lens`` (integers ``[B]`` on the device): states 0 .. kv_lens[b] - 1 of sequence b count.  ``key_mask`` (bool or
     uint8 ``[B, Lk]``): the states that count, together with the lengths.  A state that does not count contributes nothing,
     whatever its memory holds, and gets zero gradients; a query that no state counts for gets zeros.  Differentiable once in
-    q, k and v; both directions are bit-reproducible.  One query per sequence is the same call (the states are split over the chip)."""
-    what = "cross_attention"
-    q = _token_heads(what, "q", q)
-    k, v = _token_heads(what, "k", k, q.dtype), _token_heads(what, "v", v, q.dtype)
-    B, _, Hq, D = q.shape
-    Bk, Lk, Hk, Dk = k.shape
-    if k.shape != v.shape:
-        raise RuntimeError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    if Bk != B or Dk != D or Hq % Hk:
-        raise RuntimeError(f"{what}: states {tuple(k.shape)} do not fit queries {tuple(q.shape)} (same batch and channels, query "
-                           "heads a multiple of the states' heads)")
-    scale = float(D) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 1e38:
-        raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
-    if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8) or tuple(key_mask.shape) != (B, Lk):
-            raise RuntimeError(f"{what}: key_mask must be bool or uint8 {(B, Lk)}, got {key_mask.dtype} {tuple(key_mask.shape)}")
-    if kv_lens is not None:
-        if kv_lens.dtype not in (torch.int32, torch.int64) or tuple(kv_lens.shape) != (B,):
-            raise RuntimeError(f"{what}: kv_lens must be int32 or int64 {(B,)}, got {kv_lens.dtype} {tuple(kv_lens.shape)}")
-    nat.require_device(q, k, v, key_mask, kv_lens)
-    if kv_lens is not None:
-        if kv_lens.dtype != torch.int32:
-            kv_lens = kv_lens.clamp(0, Lk).int()
-        kv_lens = kv_lens.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttention.apply(q, k, v, key_mask, kv_lens, scale)
-    return _attn_forward(q, k, v, key_mask, kv_lens, scale, False)[0]
-
-
-@functools.lru_cache(maxsize=64)
-def _turn_fractions(ra, base):
-    """Turns per unit of position of the ra / 2 frequencies, as 64-bit fractions of a turn (a host array; kept alive by the cache)."""
-    f = [int(round(base ** (-2.0 * j / ra) / (2.0 * math.pi) * 2.0 ** 64)) % 2 ** 64 for j in range(ra // 2)]
-    return (C.c_uint64 * max(1, len(f)))(*f)
-
-
-def _norm_desc(q, k, wq, wk, pq, pk, rot, axes, base, eps, interleaved):
-    B, Lq, Hq, D = q.shape
-    freq = _turn_fractions(rot // axes, base)
-    d = nat.QkNormDesc(q=q.data_ptr(), freq=C.addressof(freq), B=B, Lq=Lq, Hq=Hq, Hk=1, D=D, dtype=_ATTN_TYPES[q.dtype], axes=axes,
-                       rot=rot, interleaved=interleaved, eps=eps)
-    d.keep = freq                                     # (the cache may drop the table while a graph still holds the descriptor)
-    d.q_stride[:] = q.stride()[:3]
-    if k is not None:
-        d.k, d.Lk, d.Hk = k.data_ptr(), k.shape[1], k.shape[2]
-        d.k_stride[:] = k.stride()[:3]
-    if wq is not None:
-        d.q_weight = wq.data_ptr()
-    if wk is not None:
-        d.k_weight = wk.data_ptr()
-    if pq is not None:
-        d.q_pos, d.pos64 = pq.data_ptr(), pq.dtype is torch.int64
-        if pq.dim() == 3:
-            d.q_pos_stride = pq.stride(0)
-    if pk is not None:
-        d.k_pos, d.pos64 = pk.data_ptr(), pk.dtype is torch.int64
-        if pk.dim() == 3:
-            d.k_pos_stride = pk.stride(0)
-    return d
-
-
-def _norm_forward(q, k, wq, wk, pq, pk, cfg):
-    d = _norm_desc(q, k, wq, wk, pq, pk, *cfg)
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    nat.check(nat.lib().mvf_qk_norm_rope_fwd(C.byref(d), yq.data_ptr(), _addr(yk), _raw_stream()), "qk_norm_rope_fwd")
-    return yq, yk, d
-
-
-class QkNormRope(torch.autograd.Function):
-    """Norm of every query / key head and rotation by position in one pass (csrc/mvf_qknorm.hip).  No counterpart in the reference."""
-
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, pq, pk, cfg):
-        yq, yk, d = _norm_forward(q, k, wq, wk, pq, pk, cfg)
-        ctx.save_for_backward(q, k, wq, wk, pq, pk)
-        ctx.cfg, ctx.desc = cfg, d
-        return yq if k is None else (yq, yk)
-
-    @staticmethod
-    def backward(ctx, gyq, gyk=None):
-        _once("qk_norm_rope")
-        q, k, wq, wk, pq, pk = saved = ctx.saved_tensors
-        lib, need, d, dev = nat.lib(), ctx.needs_input_grad, ctx.desc, q.device
-        if (d.q, d.k, d.q_weight, d.k_weight, d.q_pos, d.k_pos) != tuple(_addr(t) for t in saved):
-            d = _norm_desc(*saved, *ctx.cfg)
-        ref = C.byref(d)
-        gyq = _aligned(gyq, q.dtype)
-        gq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        gk = None
-        if k is not None:
-            gyk = _aligned(gyk, q.dtype)
-            gk = torch.empty(k.shape, dtype=q.dtype, device=dev)
-        gwq = torch.empty_like(wq) if need[2] else None
-        gwk = torch.empty_like(wk) if need[3] else None
-        ws = None
-        if need[2] or need[3]:
-            n = lib.mvf_qk_norm_rope_bwd_workspace_floats(ref)
-            ws = torch.empty(max(1, n), dtype=torch.float32, device=dev)
-        nat.check(lib.mvf_qk_norm_rope_bwd(ref, gyq.data_ptr(), _addr(gyk), gq.data_ptr(), _addr(gk), _addr(gwq), _addr(gwk), _addr(ws),
-                                           _raw_stream()), "qk_norm_rope_bwd")
-        return gq if need[0] else None, gk if need[1] else None, gwq, gwk, None, None, None
+    q, k and v; both directions are bit-reproducible.  One query per sequence is the same call (the states are split over the chip).
+    float32: infinities among the values that count come out as infinities or NaN."""
+    return nat.torch_ops().cross_attention(q, k, v, scale, key_mask, kv_lens)
 
 
 def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, q_pos=None, k_pos=None, *, rot_dim=None, base=10000.0, eps=1e-6,
                  interleaved=False):
-    """RMS norm of every query and key head, ``x * rsqrt(mean(x^2) + eps) * weight``, and rotation by position, in one pass.
+    """RMS norm of every query and key head, ``x * rsqrt(mean(x^2) + eps) * weight``, and rotation by position, in one pass
+    (csrc/mvf_qknorm.hip).  No counterpart in the reference.
 
     ``q [B, Lq, Hq, D]``, ``k [B, Lk, Hk, D]`` or None (queries alone: the states of an encoder are normed and rotated once); float32
     or bfloat16, D <= 128, any strides (channels adjacent; otherwise copied).  Returns ``(q', k')`` or ``q'``, contiguous.
@@ -2103,55 +1911,4 @@ def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, q_pos=None, k_pos=None
     coordinate; pair j of a block of n channels turns by ``pos * base^(-2 j / n)``; pairs are (j, j + n/2) of the block, or
     (2j, 2j + 1) if ``interleaved``.  Positions may be any integers, also negative ones: angles do not lose precision far out.
     Differentiable once in q, k and the weights; both directions are bit-reproducible."""
-    what = "qk_norm_rope"
-    q = _token_heads(what, "q", q)
-    B, Lq, _, D = q.shape
-    if k is not None:
-        k = _token_heads(what, "k", k, q.dtype)
-        if k.shape[0] != B or k.shape[3] != D:
-            raise RuntimeError(f"{what}: k {tuple(k.shape)} does not fit q {tuple(q.shape)} (same batch and channels)")
-    elif k_weight is not None or k_pos is not None:
-        raise RuntimeError(f"{what}: k_weight / k_pos without k")
-    axes = None
-    if q_pos is not None:
-        q_pos = _positions(what, "q_pos", q_pos, B, Lq)
-        axes = q_pos.shape[-1]
-    if k_pos is not None:
-        k_pos = _positions(what, "k_pos", k_pos, B, k.shape[1])
-        if axes not in (None, k_pos.shape[-1]):
-            raise RuntimeError(f"{what}: q_pos and k_pos have different numbers of axes")
-        axes = k_pos.shape[-1]
-        if q_pos is not None and q_pos.dtype != k_pos.dtype:
-            q_pos, k_pos = q_pos.long(), k_pos.long()
-    axes = axes or 1
-    rot = D // (2 * axes) * (2 * axes) if rot_dim is None else int(rot_dim)
-    if rot < 0 or rot > D or rot % (2 * axes):
-        raise RuntimeError(f"{what}: rot_dim {rot} must be a multiple of {2 * axes} (two per axis) of at most {D} channels")
-    base, eps = float(base), float(eps)
-    if not 0.0 < base < math.inf or not 0.0 <= eps < math.inf:
-        raise RuntimeError(f"{what}: base must be positive and eps not negative, got {base} and {eps}")
-    if q_weight is not None:
-        q_weight = _head_weight(what, "q_weight", q_weight, q.dtype, D)
-    if k_weight is not None:
-        k_weight = _head_weight(what, "k_weight", k_weight, q.dtype, D)
-    nat.require_device(q, k, q_weight, k_weight, q_pos, k_pos)
-    cfg = (rot, axes, base, eps, bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return QkNormRope.apply(q, k, q_weight, k_weight, q_pos, k_pos, cfg)
-    yq, yk, _ = _norm_forward(q, k, q_weight, k_weight, q_pos, k_pos, cfg)
-    return yq if k is None else (yq, yk)
-
-
-def _positions(what, name, p, B, L):
-    if p.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"{what}: {name} must be int32 or int64, got {p.dtype}")
-    p = p[:, None] if p.dim() == 1 else p
-    if p.dim() not in (2, 3) or p.shape[-2] != L or (p.dim() == 3 and p.shape[0] != B) or not 1 <= p.shape[-1] <= 3:
-        raise RuntimeError(f"{what}: {name} must be [{L}, axes] or [{B}, {L}, axes] with 1..3 axes, got {tuple(p.shape)}")
-    return p.contiguous()
-
-
-def _head_weight(what, name, w, dtype, D):
-    if w.dtype not in (torch.float32, dtype) or tuple(w.shape) != (D,):
-        raise RuntimeError(f"{what}: {name} must be [{D}] in float32 or {dtype}, got {w.dtype} {tuple(w.shape)}")
-    return w.float().contiguous()
+    return nat.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, rot_dim, base, eps, interleaved)
