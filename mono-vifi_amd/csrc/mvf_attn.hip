@@ -104,6 +104,8 @@ MVF_DEV f32x16 mma(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
+constexpr uint32_t kNowhere = 0x80000000u;       // a byte offset behind every buffer: loads give zeros
+
 // eight channels of a row as loaded
 template <int NP>
 struct Raw;
@@ -111,7 +113,7 @@ template <>
 struct Raw<1> {
     bf16x8 x;
     MVF_DEV void zero() { x = bf16x8{}; }
-    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at) { x = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0)); }
+    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at, bool) { x = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0)); }
     MVF_DEV Frag<1> frag() const { return Frag<1>{{x}}; }
     MVF_DEV Frag<1> frag_scaled(float) const { return frag(); }
 };
@@ -119,10 +121,10 @@ template <>
 struct Raw<3> {
     f32x4 a, b;
     MVF_DEV void zero() { a = b = f32x4{}; }
-    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at)
+    MVF_DEV void load(__amdgpu_buffer_rsrc_t rs, uint32_t at, bool more)      // more: the row has the last four channels too
     {
         a = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0));
-        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 16, 0, 0));
+        b = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, more ? at + 16 : kNowhere, 0, 0));
     }
     MVF_DEV Frag<3> frag() const
     {
@@ -140,7 +142,7 @@ struct Raw<3> {
 template <int NP>
 MVF_DEV float exponent(float s, float c, float minus) { return NP == 3 ? s + minus : fmaf(s, c, minus); }
 // channels d0 .. d0 + 7 of a row of D channels (zeros behind D, or if the row is not `live`); `wide`: rows are 16-byte aligned
-// and D is a multiple of 8
+// and whole 16-byte runs
 MVF_DEV Raw<1> load8(const __bf16 *row, int d0, int D, bool wide, bool live)
 {
     Raw<1> r;
@@ -163,7 +165,7 @@ MVF_DEV Raw<3> load8(const float *row, int d0, int D, bool wide, bool live)
     if (wide) {
         if (d0 < D) {
             r.a = *(const f32x4 *)(row + d0);
-            r.b = *(const f32x4 *)(row + d0 + 4);
+            if (d0 + 4 < D) r.b = *(const f32x4 *)(row + d0 + 4);
         }
     } else {
 #pragma unroll
@@ -284,7 +286,6 @@ MVF_DEV uint64_t live_states(const AttnArgs &a, int b, int j0, int n, int lane)
 // same in every lane; rows that are not valid(row) become zeros), commit() puts them into the tile.  The loads of a tile are
 // issued before the products of the one before it.  WIDE: 16-byte buffer loads, whose bounds check makes the zeros -- no branch,
 // so that all of a tile's loads are in flight at once; the host has checked that 32-bit byte offsets reach the rows of a tile.
-constexpr uint32_t kNowhere = 0x80000000u;
 template <int NP, int ROWS, int DP, bool WIDE>
 struct Flight {
     typedef typename Elem<NP>::T T;
@@ -303,7 +304,7 @@ struct Flight {
                 const bool in = (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) && chan_of(i) < D;
                 uint32_t at = in ? (uint32_t)(off(i, row_of(i)) + chan_of(i)) * (uint32_t)sizeof(T) : kNowhere;
                 if (!all && !valid(row_of(i))) at = kNowhere;
-                r[i].load(rs, at);
+                r[i].load(rs, at, chan_of(i) + 4 < D);
             }
         } else {
 #pragma unroll
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, WIDE || (a.D & 7) == 0, h);
+    store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, (a.D & 3) == 0, h);
     if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -644,12 +645,12 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int d = 16 * s + 8 * h;
-                rk[s].load(sk, mine && d < a.D ? (uint32_t)(col * ks + d) * (uint32_t)sizeof(T) : kNowhere);
+                rk[s].load(sk, mine && d < a.D ? (uint32_t)(col * ks + d) * (uint32_t)sizeof(T) : kNowhere, d + 4 < a.D);
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = i * 64 + lane, row = c / (DP / 8), d = (c - row * (DP / 8)) * 8;
-                rv[i].load(sv, ((bits >> row) & 1) && d < a.D ? (uint32_t)(row * vs + d) * (uint32_t)sizeof(T) : kNowhere);
+                rv[i].load(sv, ((bits >> row) & 1) && d < a.D ? (uint32_t)(row * vs + d) * (uint32_t)sizeof(T) : kNowhere, d + 4 < a.D);
             }
         } else {
 #pragma unroll
@@ -746,7 +747,7 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
             for (int i = 0; i < 4; ++i)
                 if (f[w] != 0.0f) x[i] = fmaf(out[(w * 32 + r) * LO + d + i], f[w], x[i]);
         if (a.splits > 1) store4(a.part + y * a.D, d, a.D, (a.D & 3) == 0, x[0], x[1], x[2], x[3]);
-        else store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, WIDE || (a.D & 7) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        else store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 3) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
     if ((threadIdx.x & 7) == 0) {
         if (a.splits > 1) {
@@ -782,7 +783,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int r = (tile * 4 + wave) * 32 + col;
-    const bool live = r < a.R, dwide = WIDE || (a.D & 7) == 0;
+    const bool live = r < a.R, dwide = WIDE || a.D % (16 / (int)sizeof(T)) == 0;      // whole 16-byte runs in the dense rows
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
     Walk<BK> w(a, b, part, lane);
@@ -870,7 +871,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
         store_cols<DT>(a.part + y * a.D, dq, a.scale, a.D, (a.D & 3) == 0, h);
         return;
     }
-    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, dwide, h);
+    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, (a.D & 3) == 0, h);
 }
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
@@ -888,7 +889,6 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     id /= a.tiles;
     const int part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
     const int j = (tile * 4 + wave) * 32 + col, n = states_of(a, b);
-    const bool dwide = WIDE || (a.D & 7) == 0;
     const int r1 = tile * 128 < n ? (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ) : 0;
     int r0 = part * a.per * BQ;
     Flight<NP, BQ, DP, WIDE> fq, fg;
@@ -988,8 +988,8 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
         return;
     }
     const int64_t y = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
-    store_cols<DT>((T *)a.dk + y, dk, a.scale, a.D, dwide, h);
-    store_cols<DT>((T *)a.dv + y, dv, 1.0f, a.D, dwide, h);
+    store_cols<DT>((T *)a.dk + y, dk, a.scale, a.D, (a.D & 3) == 0, h);
+    store_cols<DT>((T *)a.dv + y, dv, 1.0f, a.D, (a.D & 3) == 0, h);
 }
 
 // ------------------------------------------------------------------------------------------------- joining parts
@@ -1048,7 +1048,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     const float inv = MODE == 0 ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
     T *dst = MODE == 2 ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D
                        : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
-    store4(dst, d, a.D, (a.D & 7) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    store4(dst, d, a.D, (a.D & 3) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     if (MODE == 0 && a.lse && c == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -1080,7 +1080,7 @@ constexpr int kMaxGroup = 65536;
 bool wide_rows(const mvf_attn_desc &d)
 {
     const int64_t align = d.dtype == MVF_DTYPE_BF16 ? 8 : 4, G = d.Hq / d.Hk, most = 0x7fffffffLL / 4 - 128;
-    if (d.D % 8 || G > kMaxGroup) return false;
+    if (d.D % align || G > kMaxGroup) return false;
     for (int i = 0; i < 3; ++i)
         if (d.q_stride[i] % align || d.k_stride[i] % align || d.v_stride[i] % align) return false;
     if (((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) & 15) return false;

@@ -180,7 +180,53 @@ def test_strides(dtype, shape):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
-@pytest.mark.parametrize("shape", [(1, 1, 9000, 8, 2, 64), (2, 4, 5001, 4, 4, 80), (1, 9000, 3, 2, 1, 32), (1, 3000, 40, 2, 2, 128)], ids=str)
+@pytest.mark.parametrize("shape", [(2, 90, 200, 4, 2, 28), (2, 40, 130, 6, 2, 64), (1, 33, 70, 4, 4, 128), (2, 3, 300, 4, 2, 100)], ids=str)
+def test_packed_projections(dtype, shape):
+    """Keys and values as halves of one projection (16-byte loads with strides), with a mask and lengths."""
+    B, Lq, Lk, Hq, Hk, D = shape
+    q, _, _, go = make(16, dtype, *shape)
+    kv = make(17, dtype, B, Lk, 1, 2 * Hk, 1, D)[0]
+    mask = torch.rand(B, Lk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(18)) > 0.3
+    lens = torch.tensor([Lk - 5] * B, dtype=torch.int32, device="cuda")
+    check_attention(q, kv[:, :, :Hk], kv[:, :, Hk:], go, mask, lens)
+
+
+@gpu
+@pytest.mark.parametrize("stride", [1 << 22, 1 << 25], ids=["wide", "narrow"])
+def test_states_far_apart(stride):
+    """States whose byte offsets pass 32 bits, within the reach of a tile's 32-bit offsets (2^22 elements a state) and beyond it."""
+    Lk = (1 << 33) // (2 * stride) + 9                                       # a little over 8 GiB of bf16
+    q, k0, v0, go = make(19, torch.bfloat16, 1, 40, Lk, 1, 1, 64)
+    store = torch.empty(Lk * stride, dtype=torch.bfloat16, device="cuda")
+    k, v = (torch.as_strided(store, (1, Lk, 1, 64), (0, stride, 64, 1), 64 * i) for i in range(2))
+    k.copy_(k0)
+    v.copy_(v0)
+    check_attention(q, k, v, go)
+    check_attention(q[:, :1], k, v, go[:, :1])
+
+
+@gpu
+def test_saved_tensors_may_travel():
+    """Saved-tensor hooks: what the backward unpacks lies elsewhere, with other strides."""
+    q, k, v, go = make(20, torch.float32, 2, 40, 70, 4, 2, 32, strided=True)
+    w = torch.linspace(0.5, 1.5, 32, device="cuda")
+    pos = positions(20, 40, 1)
+
+    def grads():
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v, w)]
+        out = ops.cross_attention(ops.qk_norm_rope(leaves[0], None, leaves[3], q_pos=pos), leaves[1], leaves[2])
+        return torch.autograd.grad(out, leaves, go)
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    # (packed keys become contiguous: the same products by other loads)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1, 9000, 8, 2, 64), (2, 4, 5001, 4, 4, 80), (1, 9000, 3, 2, 1, 32), (1, 3000, 40, 2, 2, 128),
+                                   (1, 7, 700, 4, 2, 128), (1, 16, 333, 4, 2, 100), (3, 2, 130, 2, 2, 27)], ids=str)
 def test_few_queries_and_few_states(dtype, shape):
     """The axis that is split over the chip and joined: states for few queries, rows for few states."""
     check_attention(*make(5, dtype, *shape))
