@@ -993,16 +993,18 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 }
 
 // ------------------------------------------------------------------------------------------------- joining parts
-// A wave per row: `per` lanes hold four channels each, 64 / per groups of lanes take every (64 / per)-th part, and a butterfly
-// adds the groups: one fixed order.  (A lane that walked 60 parts by itself took 56 us of a single-token call.)
+// `wpr` waves per row (four where rows are few, else one): `per` lanes hold four channels each, the groups of lanes of all its
+// waves take the parts in turn, a butterfly adds the groups of a wave and LDS the waves: one fixed order.  (A lane that walked
+// 60 parts by itself took 56 us of a single-token call, a wave per row 11 us of 42 parts of 80 channels.)
 //   MODE 0: o = sum_p o_p 2^(m_p - m) / sum_p l_p 2^(m_p - m), and the row's lse
 //   MODE 1: dq = sum_p dq_p;  MODE 2: dk and dv, part[p][2][B * Hk][Lk][D]
 template <typename T, int MODE>
-__global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int64_t total)
+__global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int wpr, int64_t total)
 {
-    const int lane = threadIdx.x & 63, c = lane & (per - 1), pg = lane / per, groups = 64 / per, d = 4 * c;
-    const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
-    if (row >= total) return;
+    __shared__ f32x4 wave_o[3][32];
+    const int wave = threadIdx.x >> 6, sub = wave & (wpr - 1), lane = threadIdx.x & 63, c = lane & (per - 1), pg = lane / per, groups = 64 / per, d = 4 * c;
+    const int64_t row = (int64_t)blockIdx.x * (NT / 64 / wpr) + wave / wpr;
+    if (row >= total) return;                                    // (the waves of a row together)
     const int len = MODE == 2 ? a.Lk : a.R;
     const int64_t rows = (int64_t)a.B * a.Hk * len;
     const int which = MODE == 2 && row >= rows;
@@ -1024,7 +1026,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     const int64_t step = (MODE == 2 ? 2 : 1) * rows * a.D;
     const float *src = a.part + (which * rows + w) * a.D + d;
 #pragma unroll 8
-    for (int p0 = 0; p0 < a.splits; p0 += groups) {
+    for (int p0 = sub * groups; p0 < a.splits; p0 += groups * wpr) {
         const int p = p0 + pg;
         const float wt = MODE == 0 ? __shfl(f, p & 63, 64) : 1.0f;
         if (p < a.splits && d < a.D && wt != 0.0f) {
@@ -1043,6 +1045,15 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     for (int x = per; x < 64; x <<= 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], x, 64);
+    if (wpr > 1) {                                               // (per <= 32: one row per workgroup)
+        if (sub && !pg) wave_o[sub - 1][c] = f32x4{o[0], o[1], o[2], o[3]};
+        __syncthreads();
+        if (sub) return;
+#pragma unroll
+        for (int w1 = 0; w1 < 3; ++w1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += wave_o[w1][c][i];
+    }
     if (pg) return;
     const int bh = (int)(w / len), r = (int)(w - (int64_t)bh * len), b = bh / a.Hk, hk = bh - b * a.Hk;
     const float inv = MODE == 0 ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
@@ -1073,7 +1084,7 @@ void split_of(int64_t blocks, int red, int least, int &splits, int &per)
 // states of a staged tile
 constexpr int tile_states(int NP, int DP) { return NP == 1 || DP <= 32 ? 64 : 32; }
 // rows of a staged tile of the dk / dv kernel
-constexpr int tile_rows(int NP, int DP) { return NP == 1 && DP <= 64 ? 64 : 32; }
+constexpr int tile_rows(int NP, int DP) { return DP <= (NP == 1 ? 64 : 32) ? 64 : 32; }
 constexpr int kMaxGroup = 65536;
 
 // whether 16-byte loads fit: aligned rows, and 32-bit byte offsets within a tile of 64 rows or states
@@ -1174,9 +1185,10 @@ void launch_join(const AttnArgs &a, int NP, int64_t rows, hipStream_t st)
 {
     int per = 1;
     while (per * 4 < a.D) per *= 2;
-    const dim3 g((unsigned)((rows + NT / 64 - 1) / (NT / 64)));
-    if (NP == 1) hipLaunchKernelGGL((k_attn_join<__bf16, MODE>), g, dim3(NT), 0, st, a, per, rows);
-    else hipLaunchKernelGGL((k_attn_join<float, MODE>), g, dim3(NT), 0, st, a, per, rows);
+    const int wpr = rows <= 4 * kCUs ? NT / 64 : 1, rpb = NT / 64 / wpr;
+    const dim3 g((unsigned)((rows + rpb - 1) / rpb));
+    if (NP == 1) hipLaunchKernelGGL((k_attn_join<__bf16, MODE>), g, dim3(NT), 0, st, a, per, wpr, rows);
+    else hipLaunchKernelGGL((k_attn_join<float, MODE>), g, dim3(NT), 0, st, a, per, wpr, rows);
 }
 #define MVF_ATTN_PICK(fn, p, ...)                                                                      \
     do {                                                                                               \
