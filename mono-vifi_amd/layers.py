@@ -281,6 +281,8 @@ class CrossAttention(nn.Module):
         num_kv_heads = num_heads if num_kv_heads is None else num_kv_heads
         if dim % num_heads or num_heads % num_kv_heads:
             raise ValueError(f"{dim} channels, {num_heads} heads and {num_kv_heads} heads of the states do not divide")
+        if dim // num_heads > 128:
+            raise ValueError(f"{dim // num_heads} channels per head; the attention takes at most 128")
         self.num_heads, self.num_kv_heads, self.head_dim, self.base = num_heads, num_kv_heads, dim // num_heads, float(base)
         self.q = nn.Linear(dim, dim, bias=bias)
         self.kv = nn.Linear(dim if states_dim is None else states_dim, 2 * num_kv_heads * self.head_dim, bias=bias)

@@ -40,7 +40,8 @@ class CrossFrame(nn.Module):
 
     def __init__(self, channels):
         super().__init__()
-        heads = next(h for h in range(8, 0, -1) if channels % h == 0 and channels // h >= 6)
+        # eight heads or fewer of at least six channels; more where heads would be wider than the attention takes (2,048 channels)
+        heads = next((h for h in [*range(8, 0, -1), *range(9, channels + 1)] if channels % h == 0 and 6 <= channels // h <= 128), 1)
         self.attn = CrossAttention(channels, heads)
         nn.init.zeros_(self.attn.proj.weight)
         nn.init.zeros_(self.attn.proj.bias)
@@ -65,7 +66,7 @@ class FusionModule(nn.Module):
         self.fusion_conv = nn.ModuleList([
             ConvBlock1x1(2 * (int(num_ch_enc[i]) + self.embedder_obj.out_dim), int(num_ch_enc[i]))
             for i in range(n - 1, -1, -1)])
-        self.attention_levels = min(n, int(getattr(args, "fusion_attention", 0)))
+        self.attention_levels = max(0, min(n, int(getattr(args, "fusion_attention", 0))))
         if self.attention_levels:
             self.cross_frame = nn.ModuleList([CrossFrame(int(num_ch_enc[n - 1 - j])) for j in range(self.attention_levels)])
 

@@ -692,6 +692,34 @@ def test_training_step_with_fusion_attention(tmp_path, amp):
     assert proj.any() and all(torch.isfinite(p).all() for p in t.models["fusion_module"].parameters())
 
 
+@pytest.mark.parametrize("channels", [18, 36, 48, 64, 80, 128, 224, 512, 1024, 2048])
+def test_heads_of_the_fusion_attention(channels):
+    """Every width of a pyramid level gets heads that the attention takes (ResNet50's coarsest level has 2,048 channels)."""
+    from mono_vifi_amd.networks.fusion_module import CrossFrame
+    m = CrossFrame(channels).attn
+    assert m.num_heads * m.head_dim == channels and 6 <= m.head_dim <= 128
+    assert m.num_heads <= 8 or channels > 8 * 128
+
+
+@gpu
+@pytest.mark.parametrize("channels", [36, 2048])
+def test_fusion_attention_of_wide_and_narrow_levels(channels):
+    from mono_vifi_amd.networks.fusion_module import CrossFrame
+    m = CrossFrame(channels).cuda()
+    torch.nn.init.normal_(m.attn.proj.weight, std=0.02)
+    f = [torch.randn(1, channels, 3, 5, device="cuda", requires_grad=True) for _ in range(4)]
+    y = m(*f)
+    assert y.shape == f[0].shape and not torch.equal(y, f[0])
+    y.square().mean().backward()
+    assert all(torch.isfinite(x.grad).all() and x.grad.any() for x in f)
+
+
+def test_the_layer_refuses_heads_that_are_too_wide():
+    from mono_vifi_amd import layers
+    with pytest.raises(ValueError, match="at most 128"):
+        layers.CrossAttention(1024, 4)
+
+
 def test_the_layer_refuses_heads_that_do_not_divide():
     from mono_vifi_amd import layers
     for args in ((50, 8), (48, 4, 3)):
