@@ -585,7 +585,7 @@ MVF_API int mvf_color_jitter(const float *img, const float *factors, const int32
 #define MVF_ATTN_MAX_D 128
 
 typedef struct mvf_attn_desc {
-    const void *q, *k, *v;          /* q [B,Lq,Hq,D], k and v [B,Lk,Hk,D]; Hq a multiple of Hk: head h reads h / (Hq/Hk) */
+    const void *q, *k, *v;          /* q [B,Lq,Hq,D], k and v [B,Lk,Hk,D]; Hq a multiple of Hk, at most 65,536 times: head h reads h / (Hq/Hk) */
     const uint8_t *key_mask;        /* nullable [B,Lk] bytes, non-zero = the state counts */
     const int32_t *kv_lens;         /* nullable [B]: states 0 .. kv_lens[b]-1 count (clamped to 0 .. Lk) */
     int64_t q_stride[3], k_stride[3], v_stride[3];
@@ -670,7 +670,7 @@ MVF_API int mvf_qk_norm_rope_bwd(const mvf_qk_norm_desc *d, const void *g_q_out,
 #define MVF_PROF_INTERLEAVE_FWD 34   /* k_interleave_fwd */
 #define MVF_PROF_SUM_ACT_FWD 35      /* k_sum_act_fwd */
 #define MVF_PROF_ATTN_FWD 36         /* k_attn_fwd (+ k_attn_join) */
-#define MVF_PROF_ATTN_BWD 37         /* k_attn_dq + k_attn_dkv (+ k_attn_sum) */
+#define MVF_PROF_ATTN_BWD 37         /* k_attn_dq + k_attn_dkv (+ k_attn_join) */
 #define MVF_PROF_QK_NORM_FWD 38      /* k_qk_norm_fwd */
 #define MVF_PROF_QK_NORM_BWD 39      /* k_qk_norm_bwd (+ k_qk_norm_dw) */
 #define MVF_PROF_COUNT 40

@@ -1101,13 +1101,13 @@ void split_of(int64_t blocks, int red, int least, int &splits, int &per)
 constexpr int tile_states(int NP, int DP) { return NP == 1 || DP <= 32 ? 64 : 32; }
 // rows of a staged tile of the dk / dv kernel
 constexpr int tile_rows(int NP, int DP) { return DP <= (NP == 1 ? 64 : 32) ? 64 : 32; }
-constexpr int kMaxGroup = 65536;
+constexpr int kMaxGroup = 65536;                                 // query heads of a head of states (k_attn_dkv divides by a product)
 
 // whether 16-byte loads fit: aligned rows, and 32-bit byte offsets within a tile of 64 rows or states
 bool wide_rows(const mvf_attn_desc &d)
 {
     const int64_t align = d.dtype == MVF_DTYPE_BF16 ? 8 : 4, G = d.Hq / d.Hk, most = 0x7fffffffLL / 4 - 128;
-    if (d.D % align || G > kMaxGroup) return false;
+    if (d.D % align) return false;
     for (int i = 0; i < 3; ++i)
         if (d.q_stride[i] % align || d.k_stride[i] % align || d.v_stride[i] % align) return false;
     if (((uintptr_t)d.q | (uintptr_t)d.k | (uintptr_t)d.v) & 15) return false;
@@ -1148,6 +1148,7 @@ bool bad_desc(const mvf_attn_desc *d)
     if (!d || d->B < 0 || d->Lq < 0 || d->Lk < 0 || d->Hq <= 0 || d->Hk <= 0 || d->Hq % d->Hk || d->D <= 0 || d->D > MVF_ATTN_MAX_D) return true;
     if (d->dtype != MVF_DTYPE_F32 && d->dtype != MVF_DTYPE_BF16) return true;
     if (!(d->scale > 0.0f) || !(d->scale * kLog2e < INFINITY)) return true;
+    if (d->Hq / d->Hk > kMaxGroup) return true;
     const int64_t G = d->Hq / d->Hk, R = G * d->Lq, bh = (int64_t)d->B * d->Hk;
     // 32-bit tile and workgroup counts (offsets into the tensors are 64-bit throughout)
     if (R > (1 << 30) || d->Lk > (1 << 30) || bh * ((R + 127) / 128 + (d->Lk + 127) / 128 + 1) * 64 > 0x7fffffffLL) return true;

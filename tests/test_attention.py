@@ -785,6 +785,22 @@ def test_norm_refuses(args, kw, match):
         ops.qk_norm_rope(*args, **kw)
 
 
+def test_groups_beyond_the_kernels_division_are_refused():
+    """The dk / dv kernel finds a row's token by a product in fp32, exact for groups of at most 65,536 heads."""
+    g, x = (torch.arange(n, dtype=torch.float64) for n in (65537, 64))
+    for G in (1, 3, 7, 63, 1000, 65535, 65536):
+        inv = (torch.ones(1) / G).float()
+        row = torch.unique(torch.cat([g[:G][:200], g[:G][-200:]]))[:, None] + x            # g0 + row, g0 < G
+        got = ((row.float() + 0.5) * inv).floor()
+        assert torch.equal(got.double(), torch.floor(row / G)), G
+    lib = nat.lib()
+    buf = (C.c_float * 64)()
+    P = C.addressof(buf) + (-C.addressof(buf)) % 16
+    d = nat.AttnDesc(q=P, k=P, v=P, B=1, Lq=1, Lk=1, Hq=65537, Hk=1, D=1, dtype=nat.DTYPE_F32, scale=1.0)
+    assert lib.mvf_cross_attention_fwd(C.byref(d), P, None, None, None) == 1
+    assert lib.mvf_cross_attention_bwd(C.byref(d), P, P, P, P, P, P, P, None) == 1
+
+
 def test_entry_points_refuse_bad_descriptors():
     """The C entry points check their arguments before the first HIP call (hipErrorInvalidValue = 1)."""
     if not __import__("os").path.exists(nat.LIB_PATH):
