@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -102,6 +103,21 @@ void once(const char *what)
     // (a second derivative through the saved inputs would be silently missing)
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward does not run under create_graph=True");
 }
+// A leaf's gradient is accumulated on the stream that was current when the first graph that still lives first used the leaf.  If that is the
+// default stream, a backward that is being captured on another would order captured work before a stream that cannot join a
+// capture, and the process ends.  Refused while it is an error that can be caught.
+void capturable(const char *what, std::initializer_list<std::pair<const Tensor *, bool>> leaves)
+{
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const c10::Stream eager = c10::hip::getDefaultHIPStream().unwrap();
+    for (const auto &[t, needed] : leaves) {
+        if (!needed || !t->defined() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto stream = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() != eager.id(), what, ": this backward is being captured while an eager graph of the same "
+                    "leaves lives on the default stream; drop its outputs, or run the eager calls on a side stream");
+    }
+}
 Tensor dense(const Tensor &like) { return at::empty(like.sizes(), like.options(), at::MemoryFormat::Contiguous); }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor or_none(const std::optional<Tensor> &t) { return t && t->defined() ? *t : Tensor(); }
@@ -151,6 +167,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
         const mvf_attn_desc d = attn_desc(q, k, v, s[3], s[4], ctx->saved_data["scale"].toDouble());
         const Tensor g = aligned(grads[0], q.scalar_type()), out = aligned(s[5], q.scalar_type()), lse = s[6].contiguous();
         const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
+        capturable("cross_attention", {{&q, need_q}, {&k, need_k}, {&v, need_v}});
         Tensor gq = dense(q), gk, gv;
         if (need_k || need_v) { gk = dense(k); gv = dense(v); }
         const Tensor ws = at::empty({(int64_t)api.attn_bwd_bytes(&d)}, q.options().dtype(at::kByte));
@@ -269,6 +286,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
         const int ek = 1, ewq = ek + k.defined(), ewk = ewq + wq.defined();
         const bool need_k = k.defined() && ctx->needs_input_grad(ek), need_wq = wq.defined() && ctx->needs_input_grad(ewq),
                    need_wk = wk.defined() && ctx->needs_input_grad(ewk);
+        capturable("qk_norm_rope", {{&q, ctx->needs_input_grad(0)}, {&k, need_k}, {&wq, need_wq}, {&wk, need_wk}});
         if (need_wq) gwq = dense(wq);
         if (need_wk) gwk = dense(wk);
         if (need_wq || need_wk) ws = at::empty({(int64_t)api.norm_bwd_floats(&d) + 1}, q.options().dtype(at::kFloat));

@@ -1893,7 +1893,8 @@ def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
     the scores.  ``kv_lens`` (integers ``[B]`` on the device): states 0 .. kv_lens[b] - 1 of sequence b count.  ``key_mask`` (bool or
     uint8 ``[B, Lk]``): the states that count, together with the lengths.  A state that does not count contributes nothing,
     whatever its memory holds, and gets zero gradients; a query that no state counts for gets zeros.  Differentiable once in
-    q, k and v; both directions are bit-reproducible.  One query per sequence is the same call (the states are split over the chip).
+    q, k and v; both directions are bit-reproducible.  Captures into graphs; a captured backward is refused while an eager graph of the
+    same leaves lives on the default stream.  One query per sequence is the same call (the states are split over the chip).
     float32: infinities among the values that count come out as infinities or NaN."""
     return nat.torch_ops().cross_attention(q, k, v, scale, key_mask, kv_lens)
 

@@ -595,6 +595,37 @@ def test_two_captured_graphs_replay():
                 assert torch.equal(a, b)
 
 
+@gpu
+@pytest.mark.parametrize("which", ["attention", "norm"])
+def test_a_captured_backward_refuses_leaves_of_a_living_eager_graph(which):
+    """The eager graph's accumulation nodes sit on the default stream, which cannot join a capture: an error, before the engine gets
+    there.  Without the eager graph the same capture runs and replays."""
+    q, k, v, go = make(91, torch.float32, 1, 5, 40, 2, 2, 32)
+    w = torch.ones(32, device="cuda")
+    leaves = [x.requires_grad_(True) for x in ((q, k, v) if which == "attention" else (q, w))]
+
+    def call():
+        return ops.cross_attention(q, k, v) if which == "attention" else ops.qk_norm_rope(q, None, w)
+    eager = call()
+    want = [x.clone() for x in torch.autograd.grad(eager, leaves, go, retain_graph=True)]
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(g):
+            torch.autograd.grad(call(), leaves, go)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, leaves, go), want))
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(call(), leaves, go)
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------------------------------------ the modules that use them
 def layer_ref(m, x, states, xp, sp, allowed):
     """layers.CrossAttention in 64 bits from its parameters."""
@@ -690,6 +721,35 @@ def test_training_step_with_fusion_attention(tmp_path, amp):
         losses = t.optimisation_step(dict(batch))
         assert math.isfinite(float(losses["loss"]))
     assert proj.any() and all(torch.isfinite(p).all() for p in t.models["fusion_module"].parameters())
+
+
+def graph_worker(*args, timeout):
+    import os
+    import subprocess
+    import sys
+    p = subprocess.run([sys.executable, os.path.join(os.path.dirname(__file__), "attention_graph_worker.py"), *args],
+                       env={"MIOPEN_FIND_MODE": "FAST", **os.environ}, capture_output=True, text=True, timeout=timeout)
+    assert p.returncode == 0, p.stderr[-3000:]
+    return [line for line in p.stdout.splitlines() if line.startswith("RESULT ")][-1][len("RESULT "):]
+
+
+@gpu
+def test_the_layer_in_a_captured_graph():
+    """Every replay gives the eager result, projections and their biases' sums included (same kernels: the bar only allows the
+    libraries another order of a sum: fp32 sums of 12 * 960 terms)."""
+    assert float(graph_worker("layer", timeout=110)) <= 12 * 960 * U
+
+
+@gpu
+def test_captured_training_step_with_fusion_attention(tmp_path):
+    """--hip_graph with --fusion_attention follows the eager trainer (bars: tests/test_trainer_gpu.py, the same comparison without it)."""
+    import json
+    r = json.loads(graph_worker("step", "ResNet18", "2", "64", "96", str(tmp_path), "step", timeout=300))
+    e, g = r["eager"], r["graph"]
+    assert g["captured"] and all(math.isfinite(x) for row in g["losses"] for x in row)
+    for i, (a, b) in enumerate(zip(g["losses"], e["losses"])):
+        assert all(abs(x - y) <= (1e-4 if i < 2 else 5e-2) * abs(y) + 1e-6 for x, y in zip(a, b)), (i, a, b)
+    assert g["delta_norm"] > 0.5 * e["delta_norm"] > 0 and r["resume_equal"]
 
 
 @pytest.mark.parametrize("channels", [18, 36, 48, 64, 80, 128, 224, 512, 1024, 2048])
