@@ -18,7 +18,7 @@
 //
 // Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane.  fp32 inputs are three
 // (x = x0 + x1 + x2, each the leading 8 significand bits of what the previous left: exact), a product the six terms of
-// order <= 2: relative error ~2^-23 per product, and still 2.6 x the rate of the fp32 matrix instructions (6 x 32 cycles
+// order <= 2: relative error below 2^-21 per product, and still 2.6 x the rate of the fp32 matrix instructions (6 x 32 cycles
 // against 8 x 64 for a 32 x 32 x 16 product).
 //
 // Compiled without contraction (the library's flag); fused multiply-adds are written out.
@@ -480,7 +480,9 @@ MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, 
 
 // ------------------------------------------------------------------------------------------------- forward
 // grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x 32 rows).  Two tile buffers: the
-// loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile.
+// loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile (three planes:
+// one buffer).  Bound by the matrix and the vector units together (exponentials; in fp32 the cutting into planes): at 7,680 x
+// 15,360 x 64 bf16 of 8 heads 359 us = 670 TFLOP/s, at 1,920 x 3,840 x 32 fp32 of 48 heads 283 us = 160 TFLOP/s (960 in bf16).
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
@@ -624,7 +626,8 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 // workgroup idle, so here the waves share the rows and divide the states, 32 each in turn, every wave on its own: keys go from
 // memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
 // wave's own, the next 32 states are in flight meanwhile, and no barrier until the four partial results are joined in LDS.
-// Bound by the bytes of keys and values.  (5 rows against 40,001 fp32 states of 6 heads of 80: 92 us by row tiles.)
+// Bound by the bytes of keys and values: 3.3 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 9.4 us), 3.1 at 40,001 fp32 states (2 x
+// 3 heads of 80: 43 us, 92 by row tiles), where the cutting into planes takes its turn with the loads at one wave per SIMD.
 template <int NP, int DP, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
 {
@@ -784,7 +787,8 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
 // size -- dk and dv of 120 x 240 x 64 fp32: 4e-7 -> 1e-6 of the result.)
 constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
 
-// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T
+// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  Bound as the forward: 1,920 x 3,840 x 32 fp32 of 48 heads
+// 367 us = 185 TFLOP/s; 1,280 x 2,560 x 128 bf16 of 32 heads 119 us = 680 TFLOP/s.
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
@@ -890,7 +894,9 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 }
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
-// are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS
+// are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS.  1,920 x 3,840 x 32 fp32 of 48 heads
+// 519 us = 175 TFLOP/s, bound as the forward; 1,280 x 2,560 x 128 bf16 of 32 heads 219 us = 490 TFLOP/s: dk, dv, k and v in
+// registers leave one wave per SIMD.
 template <int NP, int DP, int BQ, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 {

@@ -13,7 +13,8 @@
 // polynomials of sine (x^9) and cosine (x^10) apply with an error below an fp32 step.  (A product in fp32 loses the angle
 // altogether at far positions: half a step of 300,000 is a sixtieth of a radian.)
 //
-// Bound by memory: 2 passes over the rows forward, 3 backward.  A group of lanes owns a token, so the sines and cosines are
+// Bound by memory: 2 passes over the rows forward, 3 backward (12 x (7,680 + 15,360) tokens of 8 x 64 bf16: 112 us = 5.1 TB/s and 203
+// us = 4.2).  A group of lanes owns a token, so the sines and cosines are
 // formed once for all its heads; a lane owns the same pairs of every head, loads them in runs of four, two or one, and the sum
 // of squares is a butterfly over the group (DPP), for all heads in flight at once.  All arithmetic is fp32; bf16 is rounded once, at the store.
 #include "mvf_common.hpp"
