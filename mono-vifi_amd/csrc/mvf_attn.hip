@@ -104,6 +104,20 @@ MVF_DEV f32x16 mma(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
+// the same for 16 x 16 tiles: 32 channels or states per product
+template <int NP>
+MVF_DEV f32x4 mma(const Frag<NP> &a, const Frag<NP> &b, f32x4 c)
+{
+    if constexpr (NP == 3) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+    }
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
 constexpr uint32_t kNowhere = 0x80000000u;       // a byte offset behind every buffer: loads give zeros
 
 // eight channels of a row as loaded
@@ -228,6 +242,24 @@ struct Tile {
             const short *a = &v[p * PLANE + row * LD + col];
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))a);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(a + 8 * LD));
+            s16x8 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[e] = lo[e]; x[4 + e] = hi[e]; }
+            f.p[p] = __builtin_bit_cast(bf16x8, x);
+        }
+        return f;
+    }
+    // the same of 16 channels d0 + (lane & 15), reduced over the first 32 rows in the order two 16-row accumulators hold them:
+    // element e of lane quarter g is row 4 g + (e & 3) + 16 (e >> 2)
+    MVF_DEV Frag<NP> cols16(int d0, int lane) const
+    {
+        const int row = 4 * (lane >> 4) + ((lane & 15) >> 2), col = d0 + 4 * (lane & 3);
+        Frag<NP> f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const short *a = &v[p * PLANE + row * LD + col];
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))a);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(a + 16 * LD));
             s16x8 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) { x[e] = lo[e]; x[4 + e] = hi[e]; }
@@ -404,6 +436,17 @@ MVF_DEV float other_half_max(float x)
 MVF_DEV float other_half_sum(float x)
 {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+// and of the lanes 16 apart
+MVF_DEV float other_row_max(float x)
+{
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+MVF_DEV float other_row_sum(float x)
+{
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 // state (or row) of accumulator element r of lane half h within a 32-tile
@@ -625,44 +668,56 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 // The same for at most 32 rows (a few queries, or one with the heads of its group): four row tiles would leave three waves of a
 // workgroup idle, so here the waves share the rows and divide the states, 32 each in turn, every wave on its own: keys go from
 // memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
-// wave's own, the next 32 states are in flight meanwhile, and no barrier until the four partial results are joined in LDS.
-// Bound by the bytes of keys and values: 3.3 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 9.4 us), 3.1 at 40,001 fp32 states (2 x
-// 3 heads of 80: 43 us, 92 by row tiles), where the cutting into planes takes its turn with the loads at one wave per SIMD.
-template <int NP, int DP, bool WIDE>
-__global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
+// wave's own, the next 32 states are in flight meanwhile, and no barrier until the partial results are joined in LDS.
+// ROWS: the rows of a product.
+constexpr int few_waves_of(int NP, int DP, int ROWS) { return ROWS == 16 && (NP == 1 || DP <= 96) ? 8 : 4; }
+template <int ROWS>
+struct AccOf;
+template <>
+struct AccOf<32> {
+    typedef f32x16 T;
+};
+template <>
+struct AccOf<16> {
+    typedef f32x4 T;
+};
+template <int NP, int DP, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
+    typedef typename AccOf<ROWS>::T Acc;
     typedef Tile<NP, 32, DP> VT;
-    constexpr int KS = DP / 16, DT = DP / 32, LO = DP + 4, NV = 32 * (DP / 8) / 64;
-    constexpr size_t kTiles = 4 * sizeof(VT), kOut = 4 * 32 * LO * sizeof(float);
+    constexpr int NW = few_waves_of(NP, DP, ROWS), STEP = 32 * NW;              // states of a turn of the workgroup
+    constexpr int HN = 64 / ROWS, NE = ROWS * ROWS / 64, KC = 8 * HN;        // lanes of a row, elements of an accumulator, channels of a product
+    constexpr int KS = DP / KC, ST = 32 / ROWS, CT = DP / ROWS, LO = DP + 4, NV = 32 * (DP / 8) / 64;
+    constexpr size_t kTiles = NW * sizeof(VT), kOut = NW * ROWS * LO * sizeof(float);
     __shared__ __attribute__((aligned(16))) char mem[kTiles > kOut ? kTiles : kOut];
-    __shared__ float wave_m[4][32], wave_l[4][32];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+    __shared__ float wave_m[NW][ROWS], wave_l[NW][ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & (ROWS - 1), h = lane / ROWS;
     const int id = xcd_run(blockIdx.x, gridDim.x), part = id % a.splits, bh = id / a.splits, b = bh / a.Hk, hk = bh - b * a.Hk;
     VT &tv = ((VT *)mem)[wave];
     const T *kb = (const T *)a.k + (int64_t)b * a.ks[0] + (int64_t)hk * a.ks[2];
     const T *vb = (const T *)a.v + (int64_t)b * a.vs[0] + (int64_t)hk * a.vs[2];
     const typename Stride<WIDE>::T ks = a.ks[1], vs = a.vs[1];
-    const int n = states_of(a, b), end = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * 128);
-    int j = part * a.per * 128 + wave * 32;
+    const int n = states_of(a, b), end = (int)min((int64_t)n, (int64_t)(part + 1) * a.per * STEP);
+    int j = part * a.per * STEP + wave * 32;
     uint32_t bits = 0;
     auto settle = [&] {                                           // on to 32 states of which one counts
-        for (; j < end; j += 128) {
+        for (; j < end; j += STEP) {
             bits = (uint32_t)live_states(a, b, j, n, lane);
             if (bits) return;
         }
     };
-    Raw<NP> rk[KS], rv[NV];
+    Raw<NP> rk[ST * KS], rv[NV];
     auto fetch = [&] {
         const T *kt = kb + (int64_t)j * a.ks[1], *vt = vb + (int64_t)j * a.vs[1];
-        const bool mine = (bits >> col) & 1;
         if constexpr (WIDE) {
             const __amdgpu_buffer_rsrc_t sk = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(kt), (short)0, 0x7fffffff, 0x00027000);
             const __amdgpu_buffer_rsrc_t sv = __builtin_amdgcn_make_buffer_rsrc((void *)uniform_ptr(vt), (short)0, 0x7fffffff, 0x00027000);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const int d = 16 * s + 8 * h;
-                rk[s].load(sk, mine && d < a.D ? (uint32_t)(col * ks + d) * (uint32_t)sizeof(T) : kNowhere, d + 4 < a.D);
+            for (int x = 0; x < ST * KS; ++x) {
+                const int row = x / KS * ROWS + col, d = KC * (x % KS) + 8 * h;
+                rk[x].load(sk, ((bits >> row) & 1) && d < a.D ? (uint32_t)(row * ks + d) * (uint32_t)sizeof(T) : kNowhere, d + 4 < a.D);
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -671,7 +726,11 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) rk[s] = load8(kt + (mine ? col * ks : 0), 16 * s + 8 * h, a.D, false, mine);
+            for (int x = 0; x < ST * KS; ++x) {
+                const int row = x / KS * ROWS + col;
+                const bool in = (bits >> row) & 1;
+                rk[x] = load8(kt + (in ? row * ks : 0), KC * (x % KS) + 8 * h, a.D, false, in);
+            }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int c = i * 64 + lane, row = c / (DP / 8), d = (c - row * (DP / 8)) * 8;
@@ -686,87 +745,112 @@ __global__ void __launch_bounds__(NT) k_attn_few(const AttnArgs a)
     const T *qrow = (const T *)a.q + (live ? row_off(a.qs, b, col, hk, a.G) : 0);
     Frag<NP> qf[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) qf[s] = load8(qrow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
-    f32x16 o[DT];
+    for (int s = 0; s < KS; ++s) qf[s] = load8(qrow, KC * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
+    Acc o[CT];
 #pragma unroll
-    for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+    for (int t = 0; t < CT; ++t) o[t] = Acc{};
+    auto across_max = [](float x) { return other_half_max(ROWS == 16 ? other_row_max(x) : x); };
+    auto state = [&](int t, int i) { return ROWS == 32 ? acc_row(i, 0) : 16 * t + i; };       // of element i of tile t, before 4 h
     float m = -INFINITY, l = 0.0f;
     while (j < end) {
         const uint32_t ok = bits >> (4 * h);
-        f32x16 s = {};
+        Acc s[ST];
 #pragma unroll
-        for (int x = 0; x < KS; ++x) s = mma(rk[x].frag(), qf[x], s);
+        for (int t = 0; t < ST; ++t) {
+            s[t] = Acc{};
+#pragma unroll
+            for (int x = 0; x < KS; ++x) s[t] = mma(rk[t * KS + x].frag(), qf[x], s[t]);
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = i * 64 + lane, row = c / (DP / 8);
             tv.put(row, c - row * (DP / 8), rv[i].frag());
         }
         __builtin_amdgcn_wave_barrier();                          // (LDS accesses of one wave are in order)
-        j += 128;
+        j += STEP;
         settle();
         if (j < end) fetch();
+        float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (!((ok >> acc_row(i, 0)) & 1)) s[i] = -INFINITY;
-        float mx = s[0];
+        for (int t = 0; t < ST; ++t)
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(other_half_max(mx) * (NP == 3 ? 1.0f : a.c), m);
+            for (int i = 0; i < NE; ++i) {
+                if (!((ok >> state(t, i)) & 1)) s[t][i] = -INFINITY;
+                mx = fmaxf(mx, s[t][i]);
+            }
+        mx = fmaxf(across_max(mx) * (NP == 3 ? 1.0f : a.c), m);
         const float sub = mx == -INFINITY ? 0.0f : mx, f = __builtin_amdgcn_exp2f(m - sub);
         m = mx;
         float lt = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, -sub));
-            lt += s[i];
-        }
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                s[t][i] = __builtin_amdgcn_exp2f(exponent<NP>(s[t][i], a.c, -sub));
+                lt += s[t][i];
+            }
         l = fmaf(l, f, lt);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < CT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= f;
-        accumulate<NP>(o, tv, 0, s, lane);
+            for (int i = 0; i < NE; ++i) o[d][i] *= f;
+        if constexpr (ROWS == 32) {
+            accumulate<NP>(o, tv, 0, s[0], lane);
+        } else {
+            const float p[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
+            const Frag<NP> pf = split8<NP>(p);
+            stream<NP, CT>([&](int i) { return tv.cols16(16 * i, lane); },
+                           [&](int i, const Frag<NP> &vf) {
+                               if constexpr (NP == 1) {
+                                   o[i] = mma(vf, pf, o[i]);
+                               } else {
+                                   const f32x4 y = mma(vf, pf, f32x4{});      // (summed on its own, as in accumulate)
+#pragma unroll
+                                   for (int e = 0; e < 4; ++e) o[i][e] += y[e];
+                               }
+                           });
+        }
         __builtin_amdgcn_wave_barrier();
     }
-    l = other_half_sum(l);
+    l = other_half_sum(ROWS == 16 ? other_row_sum(l) : l);
     __syncthreads();                                              // the value tiles are read: their memory takes the partial outputs
     float *out = (float *)mem;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < CT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *(f32x4 *)&out[(wave * 32 + col) * LO + 32 * t + 8 * i + 4 * h] = f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+        for (int i = 0; i < NE / 4; ++i)
+            *(f32x4 *)&out[(wave * ROWS + col) * LO + ROWS * t + 8 * i + 4 * h] = f32x4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
     if (h == 0) {
         wave_m[wave][col] = m;
         wave_l[wave][col] = l;
     }
     __syncthreads();
-    const int r = threadIdx.x >> 3;                               // eight lanes per row
+    constexpr int LPR = 64 * NW / ROWS;                           // lanes per row
+    const int r = threadIdx.x / LPR, c = threadIdx.x % LPR;
     if (r >= a.R) return;
-    float f[4], top = -INFINITY, sum = 0.0f;
+    float f[NW], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < NW; ++w)
         if (wave_l[w][r] != 0.0f) top = fmaxf(top, wave_m[w][r]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
         f[w] = wave_l[w][r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(wave_m[w][r] - top);
         sum = fmaf(wave_l[w][r], f[w], sum);
     }
     const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
     const float inv = a.splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-        const int d = 32 * t + 4 * (threadIdx.x & 7);
+    for (int d = 4 * c; d < DP; d += 4 * LPR) {
         f32x4 x = {};
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int w = 0; w < NW; ++w)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (f[w] != 0.0f) x[i] = fmaf(out[(w * 32 + r) * LO + d + i], f[w], x[i]);
+                if (f[w] != 0.0f) x[i] = fmaf(out[(w * ROWS + r) * LO + d + i], f[w], x[i]);
         if (a.splits > 1) store4(a.part + y * a.D, d, a.D, (a.D & 3) == 0, x[0], x[1], x[2], x[3]);
         else store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 3) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
-    if ((threadIdx.x & 7) == 0) {
+    if (c == 0) {
         if (a.splits > 1) {
             a.part2[2 * y] = top;
             a.part2[2 * y + 1] = sum;
@@ -1127,7 +1211,7 @@ struct Plan {
     bool wide;                               // 16-byte loads
     int NP, DP, BK, BQ;
     int rtiles, ktiles;                      // workgroups along the rows, along the states
-    bool few;                                // forward: at most 32 rows, the waves divide the states
+    int few;                                 // forward of at most 32 rows, the waves divide the states: 16 or 32 rows of a product; 0: more
     int fs, fper, qs, qper, ks, kper;        // parts of the reduction and tiles of a part: forward, dq (over the states), dkv (over the rows)
 };
 Plan plan_of(const mvf_attn_desc &d)
@@ -1142,9 +1226,10 @@ Plan plan_of(const mvf_attn_desc &d)
     const int64_t bh = (int64_t)d.B * d.Hk;
     p.rtiles = (R + 127) / 128;
     p.ktiles = (d.Lk + 127) / 128;
-    p.few = R <= 32;
+    p.few = R <= 16 ? 16 : R <= 32 ? 32 : 0;
     split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, 4, p.qs, p.qper);
-    if (p.few) split_of(bh, (d.Lk + 127) / 128, 2, p.fs, p.fper);
+    const int turn = 32 * few_waves_of(p.NP, p.DP, p.few);
+    if (p.few) split_of(bh, (d.Lk + turn - 1) / turn, 256 / turn, p.fs, p.fper);
     else p.fs = p.qs, p.fper = p.qper;
     split_of(bh * p.ktiles, (R + p.BQ - 1) / p.BQ, 4, p.ks, p.kper);
     return p;
@@ -1183,11 +1268,18 @@ void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
     if (a.wide) hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
     else hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
-template <int NP, int DP>
-void launch_few(const AttnArgs &a, int64_t blocks, hipStream_t st)
+template <int NP, int DP, int ROWS>
+void launch_few_rows(const AttnArgs &a, int64_t blocks, hipStream_t st)
 {
-    if (a.wide) hipLaunchKernelGGL((k_attn_few<NP, DP, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_few<NP, DP, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    const dim3 g((unsigned)blocks), b(64 * few_waves_of(NP, DP, ROWS));
+    if (a.wide) hipLaunchKernelGGL((k_attn_few<NP, DP, ROWS, true>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((k_attn_few<NP, DP, ROWS, false>), g, b, 0, st, a);
+}
+template <int NP, int DP>
+void launch_few(const AttnArgs &a, int rows, int64_t blocks, hipStream_t st)
+{
+    if (rows == 16) launch_few_rows<NP, DP, 16>(a, blocks, st);
+    else launch_few_rows<NP, DP, 32>(a, blocks, st);
 }
 template <int NP, int DP>
 void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
@@ -1258,7 +1350,7 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
-    if (p.few) MVF_ATTN_PICK(launch_few, p, a, (int64_t)d->B * d->Hk * p.fs, st);
+    if (p.few) MVF_ATTN_PICK(launch_few, p, a, p.few, (int64_t)d->B * d->Hk * p.fs, st);
     else MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
     if (p.fs > 1) launch_join<0>(a, p.NP, rows, st);
     return hip_check_launch();

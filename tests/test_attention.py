@@ -236,6 +236,23 @@ def test_few_queries_and_few_states(dtype, shape):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 1, 700, 16, 1, 128), (1, 17, 900, 1, 1, 96), (2, 4, 1000, 8, 2, 48), (1, 5, 333, 9, 3, 27), (1, 11, 515, 3, 1, 128),
+                                   (3, 2, 257, 8, 8, 30), (1, 31, 65, 2, 2, 57), (1, 33, 65, 2, 2, 64), (2, 3, 31, 5, 1, 100), (1, 1, 1, 1, 1, 1)], ids=str)
+@pytest.mark.parametrize("masked", [False, True], ids=["all", "masked"])
+def test_rows_that_fill_a_product_or_not(dtype, shape, masked):
+    """1 .. 33 rows against every width of the tiles: the forms for at most 16 and at most 32 rows and the next one."""
+    B, _, Lk = shape[:3]
+    q, k, v, _ = make(97, dtype, *shape)
+    kw = {}
+    if masked:
+        g = torch.Generator(device="cuda").manual_seed(98)
+        kw = dict(key_mask=torch.rand(B, Lk, device="cuda", generator=g) < 0.3,
+                  kv_lens=torch.randint(0, Lk + 1, (B,), device="cuda", generator=g))
+    check_attention(q, k, v, None, train=False, **kw)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 def test_scores_of_any_size(dtype):
     """Running maximum: scores rise along the states, fall, and one of them outweighs all (spread 12: scores of +-1,000)."""
     q, k, v, go = make(7, dtype, 1, 50, 300, 2, 2, 32)
