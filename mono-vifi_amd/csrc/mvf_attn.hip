@@ -669,8 +669,12 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 // workgroup idle, so here the waves share the rows and divide the states, 32 each in turn, every wave on its own: keys go from
 // memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
 // wave's own, the next 32 states are in flight meanwhile, and no barrier until the partial results are joined in LDS.
-// ROWS: the rows of a product.
-constexpr int few_waves_of(int NP, int DP, int ROWS) { return ROWS == 16 && (NP == 1 || DP <= 96) ? 8 : 4; }
+// ROWS: the rows of a product.  At most 16 rows take 16 x 16 x 32 products, half of the matrix work and of the registers of q and o.
+// Bound by the bytes of keys and values: 3.6 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 8.7 us), 3.9 at 40,001 fp32 states (2 x
+// 3 heads of 80: 35 us; 43 with 32-row products, 92 by row tiles).
+// Eight waves where the registers of 16-row products let two waves into a SIMD and the loads are fp32 (5 x 40,001 x 80: 41.6 us, 43.0
+// with four); bf16 keeps four (1 x 15,360 x 64, 4 x 2 heads: 14.1 us, 14.5 with eight, 17 with sixteen).
+constexpr int few_waves_of(int NP, int DP, int ROWS) { return NP == 3 && ROWS == 16 && DP <= 96 ? 8 : 4; }
 template <int ROWS>
 struct AccOf;
 template <>
@@ -1169,6 +1173,66 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     if (MODE == 0 && a.lse && c == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
+// The same for few parts (at most kFlat): a lane adds all parts of its four channels, without a word to the others.  (Two parts of
+// 120 x 240 x 64 fp32, 96 heads: 24.0 -> 20.3 us forward, 48.2 -> 46.3 backward; eight parts alike in both forms, sixteen 2 us slower.)
+constexpr int kFlat = 4;
+template <typename T, int MODE>
+__global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per, int64_t total)
+{
+    const int d = 4 * (threadIdx.x & (per - 1));
+    const int64_t row = (int64_t)blockIdx.x * (NT / per) + threadIdx.x / per;
+    if (row >= total || d >= a.D) return;
+    const int len = MODE == 2 ? a.Lk : a.R;
+    const int64_t rows = (int64_t)a.B * a.Hk * len;
+    const int which = MODE == 2 && row >= rows;
+    const int64_t w = which ? row - rows : row;
+    float f[kFlat], m = -INFINITY, l = 0.0f;
+    if (MODE == 0) {
+        float mp[kFlat];
+#pragma unroll
+        for (int p = 0; p < kFlat; ++p) {
+            const float *y = a.part2 + 2 * (min(p, a.splits - 1) * rows + w);
+            mp[p] = y[0];
+            f[p] = p < a.splits ? y[1] : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < kFlat; ++p)
+            if (f[p] != 0.0f) m = fmaxf(m, mp[p]);
+#pragma unroll
+        for (int p = 0; p < kFlat; ++p) {
+            const float lp = f[p];
+            f[p] = lp == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mp[p] - m);      // parts without a state that counts: weight 0
+            l = fmaf(lp, f[p], l);
+        }
+    }
+    float o[4] = {0, 0, 0, 0};
+    const bool quad = (a.D & 3) == 0;
+    const int64_t step = (MODE == 2 ? 2 : 1) * rows * a.D;
+    const float *src = a.part + (which * rows + w) * a.D + d;
+#pragma unroll
+    for (int p = 0; p < kFlat; ++p) {
+        const float wt = MODE == 0 ? f[p] : 1.0f;
+        if (p < a.splits && wt != 0.0f) {
+            const float *y = src + p * step;
+            if (quad) {
+                const f32x4 v = *(const f32x4 *)y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = fmaf(v[i], wt, o[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d + i < a.D) o[i] = fmaf(y[i], wt, o[i]);
+            }
+        }
+    }
+    const int bh = (int)(w / len), r = (int)(w - (int64_t)bh * len), b = bh / a.Hk, hk = bh - b * a.Hk;
+    const float inv = MODE == 0 ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+    T *dst = MODE == 2 ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D
+                       : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
+    store4(dst, d, a.D, quad, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (MODE == 0 && a.lse && d == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
 // ------------------------------------------------------------------------------------------------- host side
 
 // parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: as many as fit one workgroup per CU,
@@ -1300,6 +1364,12 @@ void launch_join(const AttnArgs &a, int NP, int64_t rows, hipStream_t st)
 {
     int per = 1;
     while (per * 4 < a.D) per *= 2;
+    if (a.splits <= kFlat) {
+        const dim3 g((unsigned)((rows + NT / per - 1) / (NT / per)));
+        if (NP == 1) hipLaunchKernelGGL((k_attn_join_flat<__bf16, MODE>), g, dim3(NT), 0, st, a, per, rows);
+        else hipLaunchKernelGGL((k_attn_join_flat<float, MODE>), g, dim3(NT), 0, st, a, per, rows);
+        return;
+    }
     const int wpr = rows <= 4 * kCUs ? NT / 64 : 1, rpb = NT / 64 / wpr;
     const dim3 g((unsigned)((rows + rpb - 1) / rpb));
     if (NP == 1) hipLaunchKernelGGL((k_attn_join<__bf16, MODE>), g, dim3(NT), 0, st, a, per, wpr, rows);

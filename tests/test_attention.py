@@ -236,6 +236,17 @@ def test_few_queries_and_few_states(dtype, shape):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 600, 700, 2, 2, 27), (2, 700, 600, 2, 1, 64), (2, 300, 1300, 1, 1, 96), (2, 1500, 300, 4, 4, 40)], ids=str)
+def test_a_few_parts_of_which_some_hold_nothing(dtype, shape):
+    """Two to eight parts of the states and of the rows; lengths that end in the first part, at once, or nowhere."""
+    q, k, v, go = make(96, dtype, *shape)
+    check_attention(q, k, v, go)
+    for lens in ([130, 0], [shape[2], 65]):
+        check_attention(q, k, v, go, kv_lens=torch.tensor(lens, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("shape", [(2, 1, 700, 16, 1, 128), (1, 17, 900, 1, 1, 96), (2, 4, 1000, 8, 2, 48), (1, 5, 333, 9, 3, 27), (1, 11, 515, 3, 1, 128),
                                    (3, 2, 257, 8, 8, 30), (1, 31, 65, 2, 2, 57), (1, 33, 65, 2, 2, 64), (2, 3, 31, 5, 1, 100), (1, 1, 1, 1, 1, 1)], ids=str)
 @pytest.mark.parametrize("masked", [False, True], ids=["all", "masked"])
