@@ -1237,8 +1237,9 @@ __global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per
 
 // parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: as many as fit one workgroup per CU,
 // with at least `least` tiles each, at most 64.  (More cost more in the parts' round trip through memory than the evener load
-// gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in one part, 338 in two; 192 of 480 x 960 x 32 backward: 65 and 73;
-// 72 of 333 x 1,281 x 28 fp32: 69, 46, 36, 38 us in 1, 2, 3, 5; 5 x 40,001 x 80 fp32: 59 us at 252 workgroups, 74 at 384.)
+// gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in one part, 338 in two; 16 of 480 x 9,600 x 64 bf16: 22 us in 16 parts, 27
+// in 32; 72 of 333 x 1,281 x 28 fp32: 34 us in two, 27 in three; 6 of 5 x 40,001 x 80 fp32: 41.5 us in 40, 56 in 64.  The exception,
+// 192 of 480 x 960 x 32 backward: 67 us in one, 64 in two.)
 constexpr int kCUs = 256;
 void split_of(int64_t blocks, int red, int least, int &splits, int &per)
 {
