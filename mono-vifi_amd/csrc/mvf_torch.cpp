@@ -5,7 +5,9 @@
 // lock to the engine's thread in every backward.  Here both directions run without the interpreter.  The module holds no kernel: it is
 // given the entry points of the library that the ctypes binding loaded (bind), and mono-vifi_amd/ops.py offers its functions.
 #include <torch/extension.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -98,10 +100,20 @@ Tensor aligned(Tensor g, at::ScalarType type)
     g = g.to(type).contiguous();
     return (uintptr_t)g.data_ptr() & 15 ? g.clone() : g;
 }
-void once(const char *what)
+// These functions call the kernels themselves, past torch's dispatcher.  A trace would hold the allocation of the output and not what
+// fills it, and a forward gradient of an input would be dropped: both are errors, in the call and in its backward.
+void direct(const char *what, std::initializer_list<const Tensor *> ts)
+{
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), what,
+                " cannot be traced: its kernels are called directly, the trace would not hold them");
+    for (const Tensor *t : ts)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative, and got a tensor with a forward gradient");
+}
+void once(const char *what, const variable_list &grads)
 {
     // (a second derivative through the saved inputs would be silently missing)
     TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: its backward does not run under create_graph=True");
+    for (const Tensor &g : grads) direct(what, {&g});
 }
 // A leaf's gradient is accumulated on the stream that was current when the first graph that still lives first used the leaf.  If that is the
 // default stream, a backward that is being captured on another would order captured work before a stream that cannot join a
@@ -161,7 +173,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
-        once("cross_attention");
+        once("cross_attention", grads);
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
         const mvf_attn_desc d = attn_desc(q, k, v, s[3], s[4], ctx->saved_data["scale"].toDouble());
@@ -179,6 +191,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
 Tensor cross_attention(Tensor q, Tensor k, Tensor v, std::optional<double> scale_, std::optional<Tensor> mask_, std::optional<Tensor> lens_)
 {
     const char *what = "cross_attention";
+    direct(what, {&q, &k, &v});
     q = token_heads(what, "q", q, {});
     k = token_heads(what, "k", k, q.scalar_type());
     v = token_heads(what, "v", v, q.scalar_type());
@@ -274,7 +287,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads)
     {
-        once("qk_norm_rope");
+        once("qk_norm_rope", grads);
         const auto s = ctx->get_saved_variables();
         auto &c = ctx->saved_data;
         const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3];
@@ -316,8 +329,9 @@ py::object qk_norm_rope(Tensor q, std::optional<Tensor> k_, std::optional<Tensor
                         std::optional<Tensor> pk_, std::optional<int64_t> rot_, double base, double eps, bool interleaved)
 {
     const char *what = "qk_norm_rope";
-    q = token_heads(what, "q", q, {});
     Tensor k = or_none(k_), wq = or_none(wq_), wk = or_none(wk_), pq = or_none(pq_), pk = or_none(pk_);
+    direct(what, {&q, &k, &wq, &wk});
+    q = token_heads(what, "q", q, {});
     const int64_t B = q.size(0), D = q.size(3);
     if (k.defined()) {
         k = token_heads(what, "k", k, q.scalar_type());

@@ -1895,7 +1895,8 @@ def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
     whatever its memory holds, and gets zero gradients; a query that no state counts for gets zeros.  Differentiable once in
     q, k and v; both directions are bit-reproducible.  Captures into graphs; a captured backward is refused while an eager graph of the
     same leaves lives on the default stream.  One query per sequence is the same call (the states are split over the chip).
-    float32: infinities among the values that count come out as infinities or NaN."""
+    Refused under ``torch.jit.trace`` and other tracing, and for inputs with a forward gradient: the kernels are called past the
+    dispatcher.  float32: infinities among the values that count come out as infinities or NaN."""
     return nat.torch_ops().cross_attention(q, k, v, scale, key_mask, kv_lens)
 
 
@@ -1911,5 +1912,6 @@ def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, q_pos=None, k_pos=None
     and column.  The first ``rot_dim`` channels (default: as many as ``2 * axes`` divides) are ``axes`` equal blocks, one per
     coordinate; pair j of a block of n channels turns by ``pos * base^(-2 j / n)``; pairs are (j, j + n/2) of the block, or
     (2j, 2j + 1) if ``interleaved``.  Positions may be any integers, also negative ones: angles do not lose precision far out.
-    Differentiable once in q, k and the weights; both directions are bit-reproducible."""
+    Differentiable once in q, k and the weights; both directions are bit-reproducible.  Refused while tracing and for inputs with a
+    forward gradient, as ``cross_attention``."""
     return nat.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, rot_dim, base, eps, interleaved)
