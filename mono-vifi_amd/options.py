@@ -153,7 +153,8 @@ def build_parser():
                         "stay ~20 eager launches")
     p.add_argument("--fusion_attention", type=int, default=0,
                    help="number of pyramid levels, coarsest first, whose fused features also attend to the tokens of both "
-                        "neighbour frames (layers.CrossAttention); 0 = the reference's fusion")
+                        "neighbour frames (layers.CrossAttention); 0 = the reference's fusion.  A checkpoint loads with at least as many "
+                        "levels as it was trained with")
     p.add_argument("--bucket_mb", type=float, default=32.0, help="gradient all-reduce bucket size")
     p.add_argument("--grad_exchange", type=str, default="all_reduce", choices=["all_reduce", "reduce_scatter"],
                    help="per gradient bucket: one RCCL all-reduce, or its two halves issued explicitly on "

@@ -855,8 +855,22 @@ class Trainer(HotPathLosses):
             if name not in checkpoint:
                 continue
             own = model.state_dict()
+            self._check_attention_levels(name, checkpoint[name], own)
             own.update({k: v for k, v in checkpoint[name].items() if k in own})
             model.load_state_dict(own)
+
+    @staticmethod
+    def _check_attention_levels(name, given, own):
+        """Keys that a model does not have are left out (the reference's checkpoints carry some), but not those of a trained
+        ``--fusion_attention``: without them the network computes other features than the one that was trained.  Levels that the
+        checkpoint lacks start as they are initialised, adding nothing to the fused features."""
+        saved, mine = (len({k.split(".")[1] for k in keys if k.startswith("cross_frame.")}) for keys in (given, own))
+        if saved > mine:
+            raise ValueError(f"the checkpoint's {name} was trained with --fusion_attention {saved}, this one has {mine}: loading it would "
+                             "drop trained attention")
+        if saved < mine:
+            logging.warning("the checkpoint's %s has %d levels of --fusion_attention, this one %d: the others start untrained", name,
+                            saved, mine)
 
     def load_ckpt(self):
         """Resume (reference: train.py:1138-1159)."""
