@@ -261,11 +261,10 @@ class ConvBlock1x1(nn.Module):
 # ----------------------------------------------------------------------------- token attention
 def token_positions(height, width, frames, device):
     """int32 [frames * height * width, 3]: frame, row and column of the tokens of ``frames`` (their indices, e.g. (-1, 1)), row-major
-    within a frame.  Created once per argument set (``consts.const_tensor``): callers must not modify it."""
-    key = ("token_positions", height, width, tuple(frames), str(device))
-    pos = consts.cached(key, lambda: torch.stack(torch.meshgrid(
-        torch.tensor(list(frames)), torch.arange(height), torch.arange(width), indexing="ij"), -1).reshape(-1, 3).int().to(device))
-    return pos
+    within a frame.  Created once per argument set (``consts.cached``): callers must not modify it."""
+    frames, device = tuple(frames), consts.device_of(device)
+    return consts.cached(("token_positions", height, width, frames, str(device)), lambda: torch.stack(torch.meshgrid(
+        torch.tensor(frames), torch.arange(height), torch.arange(width), indexing="ij"), -1).reshape(-1, 3).int().to(device))
 
 
 class CrossAttention(nn.Module):

@@ -142,3 +142,38 @@ def test_resume_with_fusion_attention(tmp_path):
     assert len(again.model_optimizer.state) == len(t.model_optimizer.state) > 0
     with pytest.raises(ValueError, match="--fusion_attention 2"):
         make_trainer(tmp_path, resume=True)
+
+
+# ------------------------------------------------------------------------------------------------ tensors that are made once
+def made_once():
+    from mono_vifi_amd import consts, layers
+    return [lambda d: layers.token_positions(3, 7, (-2, 5), d), lambda d: consts.const_tensor((0.125, 77.0), d)]
+
+
+def test_tensors_made_under_inference_mode_can_be_saved_for_a_backward(monkeypatch):
+    from mono_vifi_amd import consts
+    monkeypatch.setattr(consts, "_CACHE", {})
+    for make in made_once():
+        with torch.inference_mode():
+            first = make("cpu")
+        assert make("cpu") is first and not first.is_inference()
+        x = torch.ones(first.shape, requires_grad=True)
+        (g,) = torch.autograd.grad((x * first).sum(), x)
+        assert torch.equal(g, first.to(g.dtype))
+
+
+def test_a_device_without_an_index_is_the_current_one(monkeypatch):
+    """What was made for "cuda" on one GPU is not handed out on another: the key names the index."""
+    from mono_vifi_amd import consts
+    for make, key in zip(made_once(), (("token_positions", 3, 7, (-2, 5)), ((0.125, 77.0),))):
+        monkeypatch.setattr(consts, "_CACHE", {key + ("cuda:0",) + tail: "first" for tail in ((), (torch.float32,))} |
+                            {key + ("cuda:1",) + tail: "second" for tail in ((), (torch.float32,))})
+        for current, want in enumerate(("first", "second")):
+            monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+            assert make("cuda") == make(torch.device("cuda")) == make(f"cuda:{current}") == want
+
+
+def test_positions_of_frames_that_can_be_read_once():
+    from mono_vifi_amd import layers
+    pos = layers.token_positions(2, 2, (f for f in (-3, 4)), "cpu")
+    assert pos.tolist() == [[f, r, c] for f in (-3, 4) for r in range(2) for c in range(2)]
