@@ -5,6 +5,8 @@
 // lock to the engine's thread in every backward.  Here both directions run without the interpreter.  The module holds no kernel: it is
 // given the entry points of the library that the ctypes binding loaded (bind), and mono-vifi_amd/ops.py offers its functions.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -15,6 +17,7 @@
 #include <cmath>
 #include <map>
 #include <optional>
+#include <unordered_set>
 
 #include "../../include/mvf_hotpath.h"
 
@@ -117,17 +120,31 @@ void once(const char *what, const variable_list &grads)
 }
 // A leaf's gradient is accumulated on the stream that was current when the first graph that still lives first used the leaf.  If that is the
 // default stream, a backward that is being captured on another would order captured work before a stream that cannot join a
-// capture, and the process ends.  Refused while it is an error that can be caught.
-void capturable(const char *what, std::initializer_list<std::pair<const Tensor *, bool>> leaves)
+// capture, and the process ends.  Refused while it is an error that can be caught: for every leaf that this backward will reach
+// from its inputs whose gradients are needed (a leaf may lie behind a copy or a view of it).
+void capturable(const char *what, std::initializer_list<std::pair<const Tensor *, bool>> inputs)
 {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+    for (const auto &[t, needed] : inputs)
+        if (needed && t->defined()) todo.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
     const c10::Stream eager = c10::hip::getDefaultHIPStream().unwrap();
-    for (const auto &[t, needed] : leaves) {
-        if (!needed || !t->defined() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        const auto stream = node ? node->stream() : std::nullopt;
-        TORCH_CHECK(!stream || stream->id() != eager.id(), what, ": this backward is being captured while an eager graph of the same "
-                    "leaves lives on the default stream; drop its outputs, or run the eager calls on a side stream");
+    const auto *task = torch::autograd::get_current_graph_task_exec_info();        // which nodes run; empty: all
+    std::unordered_set<torch::autograd::Node *> seen;
+    while (!todo.empty()) {
+        const auto node = todo.back();
+        todo.pop_back();
+        if (!node || !seen.insert(node.get()).second) continue;
+        if (task && !task->empty()) {
+            const auto it = task->find(node.get());
+            if (it == task->end() || !it->second.should_execute()) continue;
+        }
+        if (dynamic_cast<torch::autograd::AccumulateGrad *>(node.get())) {
+            const auto stream = node->stream();
+            TORCH_CHECK(!stream || stream->id() != eager.id(), what, ": this backward is being captured while an eager graph of the same "
+                        "leaves lives on the default stream; drop its outputs, or run the eager calls on a side stream");
+        }
+        for (const auto &edge : node->next_edges()) todo.push_back(edge.function);
     }
 }
 Tensor dense(const Tensor &like) { return at::empty(like.sizes(), like.options(), at::MemoryFormat::Contiguous); }

@@ -273,7 +273,8 @@ class CrossAttention(nn.Module):
     ``x [B, Lq, dim]`` attends to ``states [B, Lk, states_dim]``: projections, RMS norm of every query and key head with the position
     rotation (``ops.qk_norm_rope``; positions int32 ``[L, axes]``, or None for the norm alone), attention
     (``ops.cross_attention``; ``num_kv_heads`` < ``num_heads`` shares states between query heads; ``key_mask`` / ``kv_lens`` say which
-    states count), output projection.  HIP device only, float32 or bfloat16 (also under autocast)."""
+    states count), output projection.  HIP device only, float32 or bfloat16 (also under autocast).  Before a backward of it is
+    captured, drop its eager outputs that were made on the default stream, as for every module of torch."""
 
     def __init__(self, dim, num_heads=8, num_kv_heads=None, states_dim=None, bias=True, base=100.0):
         super().__init__()

@@ -1894,7 +1894,7 @@ def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
     uint8 ``[B, Lk]``): the states that count, together with the lengths.  A state that does not count contributes nothing,
     whatever its memory holds, and gets zero gradients; a query that no state counts for gets zeros.  Differentiable once in
     q, k and v; both directions are bit-reproducible.  Captures into graphs; a captured backward is refused while an eager graph of the
-    same leaves lives on the default stream.  One query per sequence is the same call (the states are split over the chip).
+    leaves it reaches lives on the default stream.  One query per sequence is the same call (the states are split over the chip).
     Refused under ``torch.jit.trace`` and other tracing, and for inputs with a forward gradient: the kernels are called past the
     dispatcher.  float32: infinities among the values that count come out as infinities or NaN."""
     return nat.torch_ops().cross_attention(q, k, v, scale, key_mask, kv_lens)

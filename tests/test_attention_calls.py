@@ -177,3 +177,63 @@ def test_positions_of_frames_that_can_be_read_once():
     from mono_vifi_amd import layers
     pos = layers.token_positions(2, 2, (f for f in (-3, 4)), "cpu")
     assert pos.tolist() == [[f, r, c] for f in (-3, 4) for r in range(2) for c in range(2)]
+
+
+# ------------------------------------------------------------------------------------------------ captured backwards
+def captured_backward(kind):
+    """(call, leaves): leaves that the operators reach behind a copy, a conversion or a view."""
+    q, k, v = heads("cuda", Lq=5, Lk=40, D=32)
+    w = torch.linspace(0.5, 1.5, 32, device="cuda")
+    if kind == "weight in bfloat16":
+        leaves = [q.bfloat16().requires_grad_(True), w.bfloat16().requires_grad_(True)]
+        return lambda: ops.qk_norm_rope(leaves[0], None, leaves[1]), leaves
+    if kind == "channels not adjacent":
+        leaves = [x.transpose(1, 3).contiguous().transpose(1, 3).requires_grad_(True) for x in (q, k, v)]
+        return lambda: ops.cross_attention(*leaves), leaves
+    leaves = [q.requires_grad_(True), torch.cat([k, v], 2).requires_grad_(True)]
+    return lambda: ops.cross_attention(leaves[0], leaves[1][:, :, :2], leaves[1][:, :, 2:]), leaves
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["weight in bfloat16", "channels not adjacent", "packed projection"])
+def test_a_captured_backward_finds_the_leaves_of_a_living_eager_graph(kind):
+    """As for leaves that are the operators' own inputs: an error, and without the eager graph the same capture runs and replays."""
+    call, leaves = captured_backward(kind)
+    eager = call()
+    go = torch.ones_like(eager)
+    want = [x.clone() for x in torch.autograd.grad(eager, leaves, go, retain_graph=True)]
+    with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(call(), leaves, go)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(eager, leaves, go), want))
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(call(), leaves, go)
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_a_captured_backward_looks_only_at_leaves_that_it_reaches():
+    """An eager graph of a leaf whose gradient is not asked for does not stand in the way."""
+    q, k, v = (x.requires_grad_(True) for x in heads("cuda"))
+    eager = q * 2                                          # keeps q's accumulation node on the default stream
+    go = torch.ones_like(q)
+    want = torch.autograd.grad(ops.cross_attention(q.detach(), k, v), [k, v], go)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(ops.cross_attention(q, k, v), [k, v], go)
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert eager.requires_grad
