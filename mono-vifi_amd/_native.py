@@ -263,13 +263,21 @@ def torch_ops():
     global _torch_ops
     if _torch_ops is None:
         import importlib.util
+        import torch
         handle = lib()
-        path = os.path.join(_HERE, "lib", "_mvf_torch.so")
+        path, make = os.path.join(_HERE, "lib", "_mvf_torch.so"), "`python __graft_entry__.py` (or `make -C mono-vifi_amd/csrc torch`)"
         if not os.path.exists(path):
-            raise NativeLibraryError(f"{path} not found: run `python __graft_entry__.py` (or `make -C mono-vifi_amd/csrc`)")
+            raise NativeLibraryError(f"{path} not found: run {make}")
         spec = importlib.util.spec_from_file_location("_mvf_torch", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise NativeLibraryError(f"{path} does not load with torch {torch.__version__}: run {make}") from e
+        built, want = [(getattr(module, "abi", None), getattr(module, "torch", None)), (ABI_VERSION, torch.__version__.split("+")[0])]
+        if built != want:
+            raise NativeLibraryError(f"{path} was built for ABI {built[0]} and torch {built[1]}, this is ABI {want[0]} and torch {want[1]}: "
+                                     f"run {make}")
         module.bind({n: C.cast(getattr(handle, n), C.c_void_p).value for n in EXPORTS
                      if n.startswith(("mvf_cross_attention", "mvf_qk_norm", "mvf_error_string"))})
         _torch_ops = module

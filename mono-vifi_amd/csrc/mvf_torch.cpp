@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/version.h>
 
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
@@ -391,6 +392,8 @@ py::object qk_norm_rope(Tensor q, std::optional<Tensor> k_, std::optional<Tensor
 PYBIND11_MODULE(_mvf_torch, m)
 {
     m.def("bind", &bind);
+    m.attr("abi") = MVF_ABI_VERSION;                             // of the descriptors, and the torch, that this was compiled against
+    m.attr("torch") = TORCH_VERSION;
     m.def("cross_attention", &cross_attention);
     m.def("qk_norm_rope", &qk_norm_rope);
 }

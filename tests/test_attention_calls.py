@@ -237,3 +237,31 @@ def test_a_captured_backward_looks_only_at_leaves_that_it_reaches():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert eager.requires_grad
+
+
+# ------------------------------------------------------------------------------------------------ the build
+def make(*args):
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mono-vifi_amd", "csrc")
+    return subprocess.run(["make", "-n", "-C", csrc, "PYTHON=/nonexistent/python", *args], capture_output=True, text=True, timeout=60)
+
+
+@pytest.mark.parametrize("target", [(), ("all",), ("fast",), ("clean",)], ids=str)
+def test_the_c_library_is_built_without_python(target):
+    r = make(*target)
+    assert r.returncode == 0 and "/nonexistent" not in r.stdout + r.stderr and "mvf_torch" not in r.stdout
+    assert "/nonexistent" in make("torch").stdout                   # (the target that does need it)
+
+
+@pytest.mark.parametrize("what,change", [("ABI 15", lambda mp, nat: mp.setattr(nat, "ABI_VERSION", 99)),
+                                         ("torch 2", lambda mp, nat: mp.setattr(torch, "__version__", "1.0.0+other"))])
+def test_an_extension_of_another_build_is_not_loaded(monkeypatch, what, change):
+    from mono_vifi_amd import _native as nat
+    nat.lib()
+    monkeypatch.setattr(nat, "_torch_ops", None)
+    change(monkeypatch, nat)
+    with pytest.raises(nat.NativeLibraryError, match=f"built for .*{what}.*run "):
+        nat.torch_ops()
+    monkeypatch.undo()
+    assert nat.torch_ops() is not None
