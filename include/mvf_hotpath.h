@@ -579,7 +579,9 @@ MVF_API int mvf_color_jitter(const float *img, const float *factors, const int32
  * The attention the fusion of a frame with its neighbours can use (networks/fusion_module.py fuses them by
  * warping alone: fusion_module.py:100-130); no counterpart in the reference.  Tensors are [batch, token, head,
  * channel], channels adjacent; strides in ELEMENTS for batch, token and head; at most MVF_ATTN_MAX_D channels
- * per head; dtype MVF_DTYPE_F32 or MVF_DTYPE_BF16 for everything that is `void *`. */
+ * per head; dtype MVF_DTYPE_F32 or MVF_DTYPE_BF16 for everything that is `void *`.  Sizes whose launches would pass 2^32 - 1
+ * threads (8 to 16 million pairs of a sequence and a head of states) are refused like any bad argument; the workspace
+ * functions return 0 for them. */
 #define MVF_DTYPE_F32 0
 #define MVF_DTYPE_BF16 1
 #define MVF_ATTN_MAX_D 128

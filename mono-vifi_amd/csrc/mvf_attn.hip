@@ -1306,9 +1306,12 @@ bool bad_desc(const mvf_attn_desc *d)
     if (!(d->scale > 0.0f) || !(d->scale * kLog2e < INFINITY)) return true;
     if (d->Hq / d->Hk > kMaxGroup) return true;
     const int64_t G = d->Hq / d->Hk, R = G * d->Lq, bh = (int64_t)d->B * d->Hk;
-    // 32-bit tile and workgroup counts (offsets into the tensors are 64-bit throughout)
-    if (R > (1 << 30) || d->Lk > (1 << 30) || bh * ((R + 127) / 128 + (d->Lk + 127) / 128 + 1) * 64 > 0x7fffffffLL) return true;
-    return false;
+    // 32-bit tile counts (offsets into the tensors are 64-bit throughout)
+    if (R > (1 << 30) || d->Lk > (1 << 30) || bh > 0x7fffffffLL) return true;
+    // and launches that the runtime takes, of the forward and of both kernels of the backward (parts exist only of far fewer workgroups)
+    const Plan p = plan_of(*d);
+    const int64_t fwd = p.few ? bh * 64 * few_waves_of(p.NP, p.DP, p.few) : bh * p.rtiles * NT;
+    return fwd > kMaxThreads || bh * p.rtiles * NT > kMaxThreads || bh * p.ktiles * NT > kMaxThreads;
 }
 AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
 {

@@ -685,6 +685,8 @@ MVF_DEV float block_sum_many_lds(const float (&v)[NV], float *scratch)
     return r;
 }
 
+constexpr int64_t kMaxThreads = 0xffffffffLL;     // of a dimension of a grid: the runtime refuses more at the launch
+
 inline int hip_check_launch()
 {
     return (int)hipGetLastError();

@@ -362,7 +362,8 @@ bool bad_desc(const mvf_qk_norm_desc *d)
     return (int64_t)d->B * d->Lq * d->Hq > most || (int64_t)d->B * d->Lk * d->Hk > most;
 }
 
-// kernel arguments and which variant: returns PV, the longest run of channels (4, 2, 1) that the blocks and the rest are made of
+// kernel arguments and which variant: returns PV, the longest run of channels (4, 2, 1) that the blocks and the rest are made of; 0 if
+// the forward would be too large a launch (the backward walks its rows in fewer workgroups)
 int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
 {
     a = {};
@@ -378,6 +379,7 @@ int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
     a.lpr = 1;
     while (a.lpr < a.units) a.lpr *= 2;
     a.ragged = a.units < a.lpr || (d.D - d.rot) % (2 * PV);
+    int64_t blocks = 0;
     for (int i = 0; i < 2; ++i) {
         Side &s = a.side[i];
         s.x = i ? d.k : d.q;
@@ -396,12 +398,13 @@ int plan(const mvf_qk_norm_desc &d, NormArgs &a, bool bwd)
         s.chunks = (s.H + s.hg - 1) / s.hg;
         s.groups = tokens * s.chunks;
         s.blocks = (s.groups + gpb - 1) / gpb;
+        blocks += s.blocks;
         if (bwd) {                                             // rows of partial weight gradients: half of the workgroups, 256 .. 1,024
             const int64_t most = s.blocks / 2 < 256 ? 256 : s.blocks / 2 > kBwdBlocks ? kBwdBlocks : s.blocks / 2;
             if (s.blocks > most) s.blocks = most;
         }
     }
-    return PV;
+    return blocks * NT > kMaxThreads ? 0 : PV;
 }
 
 #define MVF_NORM_LAUNCH(fn, T, PV)                                                              \
@@ -431,11 +434,10 @@ int mvf_qk_norm_rope_fwd(const mvf_qk_norm_desc *d, void *q_out, void *k_out, vo
     if (bad_desc(d)) return (int)hipErrorInvalidValue;
     NormArgs a;
     const int PV = plan(*d, a, false);
-    if ((a.side[0].groups && !q_out) || (a.side[1].groups && !k_out) || (((uintptr_t)q_out | (uintptr_t)k_out) & 15))
+    if (!PV || (a.side[0].groups && !q_out) || (a.side[1].groups && !k_out) || (((uintptr_t)q_out | (uintptr_t)k_out) & 15))
         return (int)hipErrorInvalidValue;
     const int64_t blocks = a.side[0].blocks + a.side[1].blocks;
     if (blocks == 0) return 0;
-    if (blocks > 0x7fffffffLL) return (int)hipErrorInvalidValue;
     a.side[0].y = q_out;
     a.side[1].y = k_out;
     hipStream_t st = (hipStream_t)stream;
@@ -450,7 +452,7 @@ size_t mvf_qk_norm_rope_bwd_workspace_floats(const mvf_qk_norm_desc *d)
 {
     if (bad_desc(d)) return 0;
     NormArgs a;
-    plan(*d, a, true);
+    if (!plan(*d, a, true)) return 0;
     return (size_t)((a.side[0].blocks + a.side[1].blocks) * d->D);
 }
 
@@ -460,7 +462,7 @@ int mvf_qk_norm_rope_bwd(const mvf_qk_norm_desc *d, const void *g_q_out, const v
     if (bad_desc(d)) return (int)hipErrorInvalidValue;
     NormArgs a;
     const int PV = plan(*d, a, true);
-    if ((a.side[0].groups && (!g_q || !g_q_out)) || (a.side[1].groups && (!g_k || !g_k_out))) return (int)hipErrorInvalidValue;
+    if (!PV || (a.side[0].groups && (!g_q || !g_q_out)) || (a.side[1].groups && (!g_k || !g_k_out))) return (int)hipErrorInvalidValue;
     if (((uintptr_t)g_q | (uintptr_t)g_k | (uintptr_t)g_q_out | (uintptr_t)g_k_out) & 15) return (int)hipErrorInvalidValue;
     if ((g_q_weight || g_k_weight) && !workspace) return (int)hipErrorInvalidValue;
     const int64_t blocks = a.side[0].blocks + a.side[1].blocks;

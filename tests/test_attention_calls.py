@@ -265,3 +265,47 @@ def test_an_extension_of_another_build_is_not_loaded(monkeypatch, what, change):
         nat.torch_ops()
     monkeypatch.undo()
     assert nat.torch_ops() is not None
+
+
+# ------------------------------------------------------------------------------------------------ sizes at the limits of a launch
+def c_call(cls, **kw):
+    """A descriptor over a little host memory: what is refused is refused before anything is launched."""
+    import ctypes as C
+    buf = (C.c_uint64 * 64)()
+    P = C.addressof(buf) + (-C.addressof(buf)) % 16
+    fields = dict(q=P, k=P, B=1, Lq=1, Lk=1, Hq=1, Hk=1, D=8)
+    fields.update({"v": P, "scale": 1.0} if cls.__name__ == "AttnDesc" else {"freq": C.addressof(buf), "axes": 1, "eps": 1e-6})
+    return cls(**{**fields, **kw}), P, buf
+
+
+# a launch takes at most 2^32 - 1 threads.  Per sequence and head of states: fp32, at most 16 rows: 512 threads (256 at more than 96 channels), 32 rows: 256;
+# bf16: 256; the backward's two kernels: 256 per 128 rows and per 128 states
+@pytest.mark.parametrize("kw,most", [
+    (dict(dtype=0), (1 << 23) - 1), (dict(dtype=0, D=128), (1 << 24) - 1), (dict(dtype=0, Lq=32), (1 << 24) - 1), (dict(dtype=1), (1 << 24) - 1),
+    (dict(dtype=0, Lq=129), (1 << 23) - 1), (dict(dtype=1, Lk=257), ((1 << 24) - 1) // 3)])
+def test_attention_sizes_at_the_limit_of_a_launch(kw, most):
+    import ctypes as C
+    from mono_vifi_amd import _native as nat
+    lib = nat.lib()
+    for heads_ in (1, 8):
+        inside, P, keep = c_call(nat.AttnDesc, **kw, B=most // heads_, Hq=heads_, Hk=heads_)
+        assert lib.mvf_cross_attention_bwd_workspace_bytes(C.byref(inside)) > 0
+        beyond, P, keep = c_call(nat.AttnDesc, **kw, B=most // heads_ + 1, Hq=heads_, Hk=heads_)
+        assert lib.mvf_cross_attention_bwd_workspace_bytes(C.byref(beyond)) == 0
+        assert lib.mvf_cross_attention_fwd(C.byref(beyond), P, None, P, None) == 1
+        assert lib.mvf_cross_attention_bwd(C.byref(beyond), P, P, P, P, P, P, P, None) == 1
+
+
+# a workgroup of 256 threads takes 256 rows of one pair of channels, 64 of 4 lanes, 4 of 64
+@pytest.mark.parametrize("kw,rows", [(dict(D=2, rot=2), 256), (dict(D=32, rot=32), 64), (dict(D=128, rot=126, axes=3), 4)])
+def test_norm_sizes_at_the_limit_of_a_launch(kw, rows):
+    import ctypes as C
+    from mono_vifi_amd import _native as nat
+    lib = nat.lib()
+    most = min(((1 << 24) - 1) * rows, (1 << 30) - 1)
+    inside, P, keep = c_call(nat.QkNormDesc, **kw, k=None, Lq=most)
+    assert lib.mvf_qk_norm_rope_bwd_workspace_floats(C.byref(inside)) > 0
+    beyond, P, keep = c_call(nat.QkNormDesc, **kw, k=None, Lq=most + 1)
+    assert lib.mvf_qk_norm_rope_bwd_workspace_floats(C.byref(beyond)) == 0
+    assert lib.mvf_qk_norm_rope_fwd(C.byref(beyond), P, None, None) == 1
+    assert lib.mvf_qk_norm_rope_bwd(C.byref(beyond), P, None, P, None, None, None, None, None) == 1
