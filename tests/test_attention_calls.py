@@ -309,3 +309,103 @@ def test_norm_sizes_at_the_limit_of_a_launch(kw, rows):
     assert lib.mvf_qk_norm_rope_bwd_workspace_floats(C.byref(beyond)) == 0
     assert lib.mvf_qk_norm_rope_fwd(C.byref(beyond), P, None, None) == 1
     assert lib.mvf_qk_norm_rope_bwd(C.byref(beyond), P, None, P, None, None, None, None, None) == 1
+
+
+# ------------------------------------------------------------------------------------------------ how exact the fp32 products are
+# An fp32 value is three planes of bf16 (8 + 8 + 8 bits, cut), a product the six plane products of order <= 2.  Worst-case bounds of sums leave
+# room for a whole missing term; a relative 2-norm does not.  With all six, what is left out and the fp32 roundings of P and dS come to
+# 2e-7 of an output or gradient (the emulation below, exact sums).  The kernels' sums round about 6 D / 16 times per product and once per
+# tile of states, at random: sqrt(48 + 40) 2^-24 = 6e-7 of the result, twice that where two such sums follow each other.  So 2e-6; any one term
+# missing in any one product is 5e-6 or more in what depends on it.
+BAR = 2e-6
+TERMS = [(0, 0), (0, 1), (1, 0), (1, 1), (0, 2), (2, 0)]
+PRODUCTS = ["S", "PV", "dP", "dSK", "S of dk, dv", "PtG", "dStQ"]
+
+
+def planes(x):
+    out, x = [], x.float()
+    for _ in range(3):
+        cut = (x.contiguous().view(torch.int32) & -65536).view(torch.float32)
+        out.append(cut.double())
+        x = x - cut
+    return out
+
+
+def by_heads(q, k, v):
+    G = q.shape[2] // k.shape[2]
+    return [q.permute(0, 2, 1, 3)] + [x.permute(0, 2, 1, 3).repeat_interleave(G, 1) for x in (k, v)]
+
+
+def emulated(q, k, v, go, missing=(None, None)):
+    """[out, dq, dk, dv] of the three-plane products with exact sums; missing: (product, term of it that is left out)."""
+    def mm(name, a, b):
+        A, B = planes(a), planes(b)
+        return sum(A[i] @ B[j] for i, j in TERMS if (name, (i, j)) != missing)
+    t = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
+    fold = lambda x: x.unflatten(1, (k.shape[2], -1)).sum(2).permute(0, 2, 1, 3)  # noqa: E731
+    scale = q.shape[-1] ** -0.5
+    c = torch.tensor(scale / 0.6931471805599453, dtype=torch.float32)
+    qh, kh, vh = by_heads(q, k, v)
+    gh = go.permute(0, 2, 1, 3)
+    s = mm("S", qh * c, t(kh))
+    m = s.amax(-1, keepdim=True)
+    p = torch.exp2(s - m).float()
+    total = p.double().sum(-1, keepdim=True)
+    o = mm("PV", p, vh) / total
+    lse = m + total.log2()
+    delta = (gh.double() * o.float().double()).sum(-1, keepdim=True)
+    dp = mm("dP", gh, t(vh))
+    dq = mm("dSK", torch.exp2(s - lse) * (dp - delta), kh) * scale
+    p = torch.exp2(mm("S of dk, dv", qh, t(kh * c)) - lse)
+    return [o.permute(0, 2, 1, 3), dq.permute(0, 2, 1, 3), fold(mm("dStQ", t(p * (dp - delta)), qh)) * scale, fold(mm("PtG", t(p), gh))]
+
+
+def defined(q, k, v, go):
+    xs = [x.detach().double().requires_grad_(True) for x in (q, k, v)]
+    qh, kh, vh = by_heads(*xs)
+    p = torch.softmax(qh @ kh.transpose(-1, -2).contiguous() * q.shape[-1] ** -0.5, -1)
+    o = (p @ vh).permute(0, 2, 1, 3)
+    return [o.detach()] + list(torch.autograd.grad(o, xs, go.double()))
+
+
+def deviations(got, want):
+    return [float((a.double() - b).norm() / b.norm()) for a, b in zip(got, want)]
+
+
+def normal(seed, B, Lq, Lk, Hq, Hk, D, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(B, n, h, D, generator=g).to(device) for n, h in ((Lq, Hq), (Lk, Hk), (Lk, Hk), (Lq, Hq))]
+
+
+@pytest.mark.parametrize("shape", [(1, 130, 200, 2, 1, 32), (1, 70, 200, 2, 2, 28), (1, 20, 600, 1, 1, 128), (2, 3, 2500, 4, 1, 80)], ids=str)
+def test_the_bar_notices_a_missing_term(shape):
+    xs = normal(1, *shape)
+    want = defined(*xs)
+    assert max(deviations(emulated(*xs), want)) <= BAR / 8
+    depend = {"S": (0, 1), "PV": (0,), "dP": (1, 2), "dSK": (1,), "S of dk, dv": (2, 3), "PtG": (3,), "dStQ": (2,)}
+    for name in PRODUCTS:
+        for term in TERMS[1:]:
+            e = deviations(emulated(*xs, (name, term)), want)
+            assert max(e[i] for i in depend[name]) >= 2.5 * BAR, (name, term, e)
+
+
+FORMS = [(1, 130, 200, 2, 1), (2, 600, 700, 2, 2), (1, 8, 600, 2, 1), (2, 3, 2500, 4, 1), (1, 20, 600, 1, 1), (1, 31, 40, 1, 1)]
+
+
+@gpu
+@pytest.mark.parametrize("D", [28, 32, 57, 64, 80, 96, 100, 128])
+@pytest.mark.parametrize("form", FORMS, ids=["rows", "rows in parts", "16 rows", "16 rows in parts", "32 rows in parts", "32 rows"])
+def test_fp32_products_keep_all_their_terms(form, D):
+    q, k, v, go = normal(2, *form, D, device="cuda")
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    e = deviations([out.detach()] + list(torch.autograd.grad(out, leaves, go)), defined(q, k, v, go))
+    assert max(e) <= BAR, e
+
+
+@gpu
+def test_the_layer_in_a_captured_graph_stays_with_the_eager_one():
+    """The replays of the captured layer against eager calls: the operators' bits are equal, the libraries may sum in another order: twice
+    the random walk of the longest sum, 12 * 960 terms."""
+    from test_attention import graph_worker
+    assert float(graph_worker("layer", timeout=110)) <= 2 * (12 * 960) ** 0.5 * 2.0 ** -24
