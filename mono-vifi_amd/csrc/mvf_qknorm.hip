@@ -8,9 +8,10 @@
 // halves (j, j + ra/2) of the block.  Backward, with u = R(-pos) dy and r = rsqrt(mean(x^2) + eps):
 //     dw = sum over rows of u x r,    dx = r w u - x r^3 / D * sum(u w x)
 //
-// Angles are exact for any position: a frequency is a 64-bit fixed-point fraction of a turn, so pos * freq modulo one turn is
-// one integer product; its top bits give the quadrant and a remainder of at most an eighth of a turn, to which the Taylor
-// polynomials of sine (x^9) and cosine (x^10) apply with an error below an fp32 step.  (A product in fp32 loses the angle
+// A frequency is a 64-bit fixed-point fraction of a turn, so pos * freq modulo one turn is one integer product without an error of its
+// own; its top bits give the quadrant and a remainder of at most an eighth of a turn, to which the Taylor polynomials of sine
+// (x^9) and cosine (x^10) apply with an error below an fp32 step.  What is left is the frequency's rounding, |pos| * 2^-64 of a turn at
+// most (base >= 1): below an fp32 step up to |pos| = 2^37, 4e-7 radians at 2^40, 1e-4 at 2^48.  (A product in fp32 loses the angle
 // altogether at far positions: half a step of 300,000 is a sixtieth of a radian.)
 //
 // Bound by memory: 2 passes over the rows forward, 3 backward (12 x (7,680 + 15,360) tokens of 8 x 64 bf16: 112 us = 5.1 TB/s and 203

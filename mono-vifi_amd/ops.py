@@ -1911,7 +1911,8 @@ def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, q_pos=None, k_pos=None
     ``[B, L, axes]`` (``[L]``: one axis), or None for no rotation of that side; up to three axes -- an index; row and column; frame, row
     and column.  The first ``rot_dim`` channels (default: as many as ``2 * axes`` divides) are ``axes`` equal blocks, one per
     coordinate; pair j of a block of n channels turns by ``pos * base^(-2 j / n)``; pairs are (j, j + n/2) of the block, or
-    (2j, 2j + 1) if ``interleaved``.  Positions may be any integers, also negative ones: angles do not lose precision far out.
+    (2j, 2j + 1) if ``interleaved``.  Positions may be any integers, also negative ones: an angle is off by at most
+    ``|pos| * 2^-64`` of a turn (``base`` >= 1), which float32 does not see up to 2^37 and which grows from there.
     Differentiable once in q, k and the weights; both directions are bit-reproducible.  Refused while tracing and for inputs with a
     forward gradient, as ``cross_attention``."""
     return nat.torch_ops().qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, rot_dim, base, eps, interleaved)

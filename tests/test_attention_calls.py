@@ -409,3 +409,52 @@ def test_the_layer_in_a_captured_graph_stays_with_the_eager_one():
     the random walk of the longest sum, 12 * 960 terms."""
     from test_attention import graph_worker
     assert float(graph_worker("layer", timeout=110)) <= 2 * (12 * 960) ** 0.5 * 2.0 ** -24
+
+
+# ------------------------------------------------------------------------------------------------ far positions
+def sines(pos, n, base):
+    """Sine and cosine of pos * base^(-2 j / n), j < n / 2, from 60 digits."""
+    import decimal
+    import math
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        pi = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        out = []
+        for p in pos:
+            row = []
+            for j in range(n // 2):
+                turns = decimal.Decimal(p) * (decimal.Decimal(-2 * j) / n * decimal.Decimal(base).ln()).exp() / (2 * pi)
+                a = float((turns - turns.to_integral_value(decimal.ROUND_FLOOR)) * 2 * pi)
+                row.append((math.sin(a), math.cos(a)))
+            out.append(row)
+    return torch.tensor(out, dtype=torch.float64)                    # [L, n / 2, 2]
+
+
+def test_sines_of_near_positions_are_those_of_64_bits():
+    pos = [-70, 0, 1, 999]
+    ang = torch.tensor(pos, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, 16, 2, dtype=torch.float64) / 16)
+    # (an angle in 64 bits: the frequency and the product round, 2^-52 of up to 1,000)
+    assert (sines(pos, 16, 10000) - torch.stack([ang.sin(), ang.cos()], -1)).abs().max() <= 1000 * 2.0 ** -52
+
+
+@gpu
+@pytest.mark.parametrize("base", [10000, 100])
+@pytest.mark.parametrize("bits", [20, 31, 37, 40, 48, 62])
+def test_far_positions_are_off_by_their_frequencies_rounding_alone(bits, base):
+    """|pos| * 2^-64 of a turn, and the fp32 roundings of the norm and the rotation, (D + 24) 2^-24 of the pair (tests/test_attention.py)."""
+    import math
+    import random
+    D, rng = 32, random.Random(bits)
+    pos = [(1 << bits) - 1, 1 - (1 << bits), (1 << (bits - 1)) + 1] + [rng.randrange(-(1 << bits), 1 << bits) for _ in range(13)]
+    x = torch.randn(1, len(pos), 1, D, generator=torch.Generator().manual_seed(bits))
+    got = ops.qk_norm_rope(x.cuda(), q_pos=torch.tensor(pos, device="cuda"), base=float(base), eps=0.0)[0, :, 0].double().cpu()
+    n = x[0, :, 0].double()
+    n = n / (n * n).mean(-1, keepdim=True).sqrt()
+    a, b = n[:, :D // 2], n[:, D // 2:]
+    s, c = sines(pos, D, base).unbind(-1)
+    want = torch.cat([a * c - b * s, a * s + b * c], -1)
+    off = 2 * math.pi * torch.tensor([abs(p) for p in pos], dtype=torch.float64)[:, None] * 2.0 ** -64
+    size = (a.abs() + b.abs()).repeat(1, 2)
+    assert ((got - want).abs() <= size * ((D + 24) * 2.0 ** -24 + off) + 2.0 ** -24 * want.abs()).all()
+    # and at far positions the bound itself says something: not more than a hundredth of a radian up to 2^48
+    assert bits > 48 or float(off.max()) < 1e-2
