@@ -16,7 +16,10 @@
 // tile is a permutation of the reduction index, and V is read from LDS in the same permutation (ds_read_b64_tr_b16: four
 // states of one channel per lane), so P never moves between lanes.
 //
-// Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane.  fp32 inputs are three
+// Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane, and what becomes an operand of a
+// second product is rounded to one as well: P before V^T P and P^T do, dS before dq and dk (2^-8 of a term at most; in fp32 they would
+// take the six products below, six times the matrix work); delta = do . o takes the output as it was stored, in bf16.  Results
+// are 2.0e-3 - 2.4e-3 from the 64-bit ones (relative 2-norm), 1.7e-3 of which is the rounding of the result itself.  fp32 inputs are three
 // (x = x0 + x1 + x2, each the leading 8 significand bits of what the previous left: exact), a product the six terms of
 // order <= 2: relative error below 2^-21 per product, and still 2.6 x the rate of the fp32 matrix instructions (6 x 32 cycles
 // against 8 x 64 for a 32 x 32 x 16 product).
@@ -524,8 +527,11 @@ MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, 
 // ------------------------------------------------------------------------------------------------- forward
 // grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x 32 rows).  Two tile buffers: the
 // loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile (three planes:
-// one buffer).  Bound by the matrix and the vector units together (exponentials; in fp32 the cutting into planes): at 7,680 x
-// 15,360 x 64 bf16 of 8 heads 359 us = 670 TFLOP/s, at 1,920 x 3,840 x 32 fp32 of 48 heads 283 us = 160 TFLOP/s (960 in bf16).
+// one buffer).  (Times here and below are of kernel traces; among repeated calls the large ones are 3 - 6 % shorter.)
+// 1,920 x 3,840 x 32 fp32 of 48 heads: 281 us = 161 TFLOP/s (970 in bf16), the vector units active 0.61 of the time (exponentials, cutting
+// into planes) and the matrix units 0.46.  7,680 x 15,360 x 64 bf16 of 8 heads: 343 us = 704 TFLOP/s, vector 0.45, matrix 0.29: two waves per
+// SIMD wait, a third of their cycles for an instruction to be taken.  1,280 x 2,560 x 128 bf16 of 32 heads: 94 us = 570 TFLOP/s, both 0.2: one
+// wave per SIMD, 320 workgroups on 256 CUs.
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
@@ -670,7 +676,7 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 // memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
 // wave's own, the next 32 states are in flight meanwhile, and no barrier until the partial results are joined in LDS.
 // ROWS: the rows of a product.  At most 16 rows take 16 x 16 x 32 products, half of the matrix work and of the registers of q and o.
-// Bound by the bytes of keys and values: 3.6 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 8.7 us), 3.9 at 40,001 fp32 states (2 x
+// Bound by the bytes of keys and values: 3.8 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 8.2 us), 3.9 at 40,001 fp32 states (2 x
 // 3 heads of 80: 35 us; 43 with 32-row products, 92 by row tiles).
 // Eight waves where the registers of 16-row products let two waves into a SIMD and the loads are fp32 (5 x 40,001 x 80: 41.6 us, 43.0
 // with four); bf16 keeps four (1 x 15,360 x 64, 4 x 2 heads: 14.1 us, 14.5 with eight, 17 with sixteen).
@@ -867,6 +873,8 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 // ------------------------------------------------------------------------------------------------- backward
 // P is recomputed from the stored log2 of the softmax sum; delta = do . o is what the softmax subtracts from dP:
 //     dS = P (dP - delta),  dP = do V^T,  dq = scale dS K,  dk = scale dS^T q,  dv = P^T do
+// (delta is summed in fp32 from do and the stored output; in bf16 the output's rounding is in it, 2^-8 of |do| . |o| at most: forming it
+// from P and dP instead would take another pass over the states.)
 // Two passes without atomics, so that the sums have one order: rows own dq (and write delta), states own dk and dv.  The
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
@@ -875,8 +883,8 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 // size -- dk and dv of 120 x 240 x 64 fp32: 4e-7 -> 1e-6 of the result.)
 constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
 
-// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  Bound as the forward: 1,920 x 3,840 x 32 fp32 of 48 heads
-// 367 us = 185 TFLOP/s; 1,280 x 2,560 x 128 bf16 of 32 heads 119 us = 680 TFLOP/s.
+// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  1,920 x 3,840 x 32 fp32 of 48 heads: 364 us = 187 TFLOP/s, matrix
+// units 0.55, vector units 0.51 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 119 us = 680 TFLOP/s, 0.26 and 0.21.
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
@@ -982,9 +990,9 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 }
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
-// are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS.  1,920 x 3,840 x 32 fp32 of 48 heads
-// 519 us = 175 TFLOP/s, bound as the forward; 1,280 x 2,560 x 128 bf16 of 32 heads 219 us = 490 TFLOP/s: dk, dv, k and v in
-// registers leave one wave per SIMD.
+// are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS.  1,920 x 3,840 x 32 fp32 of 48 heads:
+// 504 us = 180 TFLOP/s, matrix units 0.53, vector units 0.54 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 218 us = 490 TFLOP/s, 0.19 and
+// 0.17: dk, dv, k and v in registers leave one wave per SIMD.
 template <int NP, int DP, int BQ, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 {
@@ -1174,7 +1182,8 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
 }
 
 // The same for few parts (at most kFlat): a lane adds all parts of its four channels, without a word to the others.  (Two parts of
-// 120 x 240 x 64 fp32, 96 heads: 24.0 -> 20.3 us forward, 48.2 -> 46.3 backward; eight parts alike in both forms, sixteen 2 us slower.)
+// 120 x 240 x 64 fp32, 96 heads: 24.0 -> 20.3 us forward, 48.2 -> 46.3 backward by events around the launches -- an eager training call
+// is the host's, 71 - 74 us either way; eight parts alike in both forms, sixteen 2 us slower.)
 constexpr int kFlat = 4;
 template <typename T, int MODE>
 __global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per, int64_t total)
@@ -1237,7 +1246,7 @@ __global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per
 
 // parts of a reduction of `red` tiles when `blocks` workgroups exist without splitting: as many as fit one workgroup per CU,
 // with at least `least` tiles each, at most 64.  (More cost more in the parts' round trip through memory than the evener load
-// gives: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in one part, 338 in two; 16 of 480 x 9,600 x 64 bf16: 22 us in 16 parts, 27
+// gives, in calls: 480 workgroups, 7,680 x 15,360 x 64 bf16: 321 us in one part, 338 in two; 16 of 480 x 9,600 x 64 bf16: 22 us in 16 parts, 27
 // in 32; 72 of 333 x 1,281 x 28 fp32: 34 us in two, 27 in three; 6 of 5 x 40,001 x 80 fp32: 41.5 us in 40, 56 in 64.  The exception,
 // 192 of 480 x 960 x 32 backward: 67 us in one, 64 in two.)
 constexpr int kCUs = 256;

@@ -14,8 +14,9 @@
 // most (base >= 1): below an fp32 step up to |pos| = 2^37, 4e-7 radians at 2^40, 1e-4 at 2^48.  (A product in fp32 loses the angle
 // altogether at far positions: half a step of 300,000 is a sixtieth of a radian.)
 //
-// Bound by memory: 2 passes over the rows forward, 3 backward (12 x (7,680 + 15,360) tokens of 8 x 64 bf16: 112 us = 5.1 TB/s and 203
-// us = 4.2).  A group of lanes owns a token, so the sines and cosines are
+// Bound by memory: 2 passes over the rows forward, 3 backward (12 x (7,680 + 15,360) tokens of 8 x 64 bf16, two axes: 111 us = 5.1 TB/s
+// and 199 us = 4.3).  Blocks of an odd number of pairs are loaded one channel at a time (three axes of 64 channels: two): 12 x (1,920 +
+// 3,840) tokens of 8 x 32 fp32, three axes: 27 us a call = 5.3 TB/s, of 8 x 16: 16 us = 4.4.  A group of lanes owns a token, so the sines and cosines are
 // formed once for all its heads; a lane owns the same pairs of every head, loads them in runs of four, two or one, and the sum
 // of squares is a butterfly over the group (DPP), for all heads in flight at once.  All arithmetic is fp32; bf16 is rounded once, at the store.
 #include "mvf_common.hpp"
