@@ -16,10 +16,10 @@
 // tile is a permutation of the reduction index, and V is read from LDS in the same permutation (ds_read_b64_tr_b16: four
 // states of one channel per lane), so P never moves between lanes.
 //
-// Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane, and what becomes an operand of a
-// second product is rounded to one as well: P before V^T P and P^T do, dS before dq and dk (2^-8 of a term at most; in fp32 they would
-// take the six products below, six times the matrix work); delta = do . o takes the output as it was stored, in bf16.  Results
-// are 2.0e-3 - 2.4e-3 from the 64-bit ones (relative 2-norm), 1.7e-3 of which is the rounding of the result itself.  fp32 inputs are three
+// Types.  Everything the matrix units multiply is bf16; sums are fp32.  bf16 inputs are one plane.  What becomes an operand of a second
+// product (P before V^T P and P^T do, dS before dq and dk) is two planes, 2^-16 of a term, where that matters or is free (kSmall, below),
+// else one, rounded: 2^-8 of a term at most.  The results of one plane (large inference outputs, dk and dv) are 2.3e-3 - 2.4e-3 from the
+// 64-bit ones (relative 2-norm), those of two 1.7e-3, which is the rounding of the result itself.  fp32 inputs are three
 // (x = x0 + x1 + x2, each the leading 8 significand bits of what the previous left: exact), a product the six terms of
 // order <= 2: relative error below 2^-21 per product, and still 2.6 x the rate of the fp32 matrix instructions (6 x 32 cycles
 // against 8 x 64 for a 32 x 32 x 16 product).
@@ -91,6 +91,21 @@ MVF_DEV Frag<NP> split8(const float (&x)[8])
         f.p[2] = __builtin_bit_cast(bf16x8, c);
     }
     return f;
+}
+
+// eight fp32 values as two planes: the leading 8 significand bits (cut), and what they leave, rounded to 8 bits.  P: of probabilities, whose
+// second plane is never zero -- an infinite value of a state that counts has to come out as an infinity, and 0 x inf is none
+template <bool P>
+MVF_DEV void split8(const float (&x)[8], Frag<1> &hi, Frag<1> &lo)
+{
+    s16x8 a;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        a[e] = top16(x[e]);
+        const float rest = x[e] - trunc_bf16(x[e]);
+        lo.p[0][e] = (__bf16)(P ? fmaxf(rest, 0x1p-126f) : rest);
+    }
+    hi.p[0] = __builtin_bit_cast(bf16x8, a);
 }
 
 // c += a b; the small terms of the three-plane product first
@@ -275,7 +290,7 @@ struct Tile {
 // ------------------------------------------------------------------------------------------------- arguments
 struct AttnArgs {
     const void *q, *k, *v, *o, *go;
-    void *out, *dq, *dk, *dv;
+    void *out, *low, *dq, *dk, *dv;           // low: what the rounding of out left (bf16 training), or null
     float *lse, *delta, *part, *part2;
     const uint8_t *mask;
     const int32_t *lens;
@@ -464,6 +479,17 @@ MVF_DEV Frag<NP> acc_frag(const f32x16 &x, int s)
     for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
     return split8<NP>(y);
 }
+template <bool P>
+MVF_DEV void acc_frag(const f32x16 &x, int s, Frag<1> &hi, Frag<1> &lo)
+{
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[8 * s + e];
+    split8<P>(y, hi, lo);
+}
+
+// what rounding to bf16 leaves of a value
+MVF_DEV float rest_bf16(float x) { return x - (float)(__bf16)x; }
 
 // four consecutive channels d .. d + 3 of a row
 MVF_DEV void store4(float *row, int d, int D, bool wide, float a, float b, float c, float e)
@@ -489,6 +515,12 @@ MVF_DEV void store4(__bf16 *row, int d, int D, bool wide, float a, float b, floa
     for (int i = 0; i < 4; ++i)
         if (d + i < D) row[d + i] = (__bf16)x[i];
 }
+// what the rounding of x f to bf16 left, rounded itself
+template <typename T>
+MVF_DEV void store_rest(T *row, int d, int D, const float (&x)[4], float f)
+{
+    store4(row, d, D, (D & 3) == 0, rest_bf16(x[0] * f), rest_bf16(x[1] * f), rest_bf16(x[2] * f), rest_bf16(x[3] * f));
+}
 // accumulator tiles (channel rows, this lane's column) -> a row of D channels, scaled
 template <int DT, typename T>
 MVF_DEV void store_cols(T *row, const f32x16 (&acc)[DT], float f, int D, bool wide, int h)
@@ -501,12 +533,33 @@ MVF_DEV void store_cols(T *row, const f32x16 (&acc)[DT], float f, int D, bool wi
                    acc[t][4 * i + 3] * f);
 }
 
-// acc[d] += (32 channels d of the tile's rows r0 .. r0 + 31)^T x.  NP == 3: the products of a tile are summed on their own and
+template <int DT, typename T>
+MVF_DEV void store_cols_rest(T *row, const f32x16 (&acc)[DT], float f, int D, int h)
+{
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x[4] = {acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]};
+            store_rest(row, 32 * t + 8 * i + 4 * h, D, x, f);
+        }
+}
+
+// acc[d] += (32 channels d of the tile's rows r0 .. r0 + 31)^T x.  TWO: x as two planes of bf16 instead of one (P: of probabilities).  NP == 3: the products of a tile are summed on their own and
 // then added to the running sum, so that its roundings are one per tile and not one per matrix instruction (3,840 states:
 // error 5e-6 -> 1e-6 of the result).
-template <int NP, int DT, int ROWS, int DP>
+template <int NP, bool TWO, bool P, int DT, int ROWS, int DP>
 MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, const f32x16 &x, int lane)
 {
+    static_assert(NP == 1 || !TWO, "");
+    if constexpr (TWO) {
+        Frag<1> hi[2], lo[2];
+        acc_frag<P>(x, 0, hi[0], lo[0]);
+        acc_frag<P>(x, 1, hi[1], lo[1]);
+        stream<NP, 2 * DT>([&](int i) { return t.cols(32 * (i % DT), r0 + 16 * (i / DT), lane); },
+                           [&](int i, const Frag<NP> &f) { acc[i % DT] = mma(f, hi[i / DT], mma(f, lo[i / DT], acc[i % DT])); });
+        return;
+    }
     const Frag<NP> xf[2] = {acc_frag<NP>(x, 0), acc_frag<NP>(x, 1)};
     if constexpr (NP == 1) {
         stream<NP, 2 * DT>([&](int i) { return t.cols(32 * (i % DT), r0 + 16 * (i / DT), lane); },
@@ -527,12 +580,12 @@ MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, 
 // ------------------------------------------------------------------------------------------------- forward
 // grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x 32 rows).  Two tile buffers: the
 // loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile (three planes:
-// one buffer).  (Times here and below are of kernel traces; among repeated calls the large ones are 3 - 6 % shorter.)
-// 1,920 x 3,840 x 32 fp32 of 48 heads: 281 us = 161 TFLOP/s (970 in bf16), the vector units active 0.61 of the time (exponentials, cutting
-// into planes) and the matrix units 0.46.  7,680 x 15,360 x 64 bf16 of 8 heads: 343 us = 704 TFLOP/s, vector 0.45, matrix 0.29: two waves per
-// SIMD wait, a third of their cycles for an instruction to be taken.  1,280 x 2,560 x 128 bf16 of 32 heads: 94 us = 570 TFLOP/s, both 0.2: one
-// wave per SIMD, 320 workgroups on 256 CUs.
-template <int NP, int DP, int BK, bool WIDE>
+// one buffer).  (Times here and below are of kernel traces; among repeated calls the large ones are 3 - 10 % shorter.)
+// 1,920 x 3,840 x 32 fp32 of 48 heads: 281 - 285 us = 160 TFLOP/s (960 in bf16), the vector units active 0.61 of the time (exponentials,
+// cutting into planes) and the matrix units 0.47.  7,680 x 15,360 x 64 bf16 of 8 heads: 343 - 359 us = 690 TFLOP/s, vector 0.45, matrix 0.30: two
+// waves per SIMD wait, a third of their cycles for an instruction to be taken.  1,280 x 2,560 x 128 bf16 of 32 heads: 94 us = 570 TFLOP/s, in
+// training (P in two planes) 117; vector 0.24, matrix 0.27: 320 workgroups on 256 CUs, one wave per SIMD.
+template <int NP, int DP, int BK, bool WIDE, bool TWO>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
@@ -649,7 +702,7 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
         first = false;
         l += lt;
 #pragma unroll
-        for (int t = 0; t < KT; ++t) accumulate<NP>(o, tv, 32 * t, s[t], lane);
+        for (int t = 0; t < KT; ++t) accumulate<NP, TWO, true>(o, tv, 32 * t, s[t], lane);
         if (kTwo) {
             buf ^= 1;
             if (w.live()) commit();
@@ -668,6 +721,7 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, (a.D & 3) == 0, h);
+    if (TWO && a.low) store_cols_rest<DT>((T *)a.low + dense_row(b, r, hk, a), o, inv, a.D, h);
     if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -691,7 +745,7 @@ template <>
 struct AccOf<16> {
     typedef f32x4 T;
 };
-template <int NP, int DP, int ROWS, bool WIDE>
+template <int NP, int DP, int ROWS, bool WIDE, bool TWO>
 __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
@@ -805,13 +859,17 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 #pragma unroll
             for (int i = 0; i < NE; ++i) o[d][i] *= f;
         if constexpr (ROWS == 32) {
-            accumulate<NP>(o, tv, 0, s[0], lane);
+            accumulate<NP, TWO, true>(o, tv, 0, s[0], lane);
         } else {
             const float p[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
-            const Frag<NP> pf = split8<NP>(p);
+            Frag<NP> pf, low;
+            if constexpr (TWO) split8<true>(p, pf, low);
+            else pf = split8<NP>(p);
             stream<NP, CT>([&](int i) { return tv.cols16(16 * i, lane); },
                            [&](int i, const Frag<NP> &vf) {
-                               if constexpr (NP == 1) {
+                               if constexpr (TWO) {
+                                   o[i] = mma(vf, pf, mma(vf, low, o[i]));
+                               } else if constexpr (NP == 1) {
                                    o[i] = mma(vf, pf, o[i]);
                                } else {
                                    const f32x4 y = mma(vf, pf, f32x4{});      // (summed on its own, as in accumulate)
@@ -858,7 +916,10 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
             for (int i = 0; i < 4; ++i)
                 if (f[w] != 0.0f) x[i] = fmaf(out[(w * ROWS + r) * LO + d + i], f[w], x[i]);
         if (a.splits > 1) store4(a.part + y * a.D, d, a.D, (a.D & 3) == 0, x[0], x[1], x[2], x[3]);
-        else store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 3) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        else {
+            store4((T *)a.out + dense_row(b, r, hk, a), d, a.D, (a.D & 3) == 0, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            if (TWO && a.low) store_rest((T *)a.low + dense_row(b, r, hk, a), d, a.D, {x[0], x[1], x[2], x[3]}, inv);
+        }
     }
     if (c == 0) {
         if (a.splits > 1) {
@@ -873,8 +934,10 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 // ------------------------------------------------------------------------------------------------- backward
 // P is recomputed from the stored log2 of the softmax sum; delta = do . o is what the softmax subtracts from dP:
 //     dS = P (dP - delta),  dP = do V^T,  dq = scale dS K,  dk = scale dS^T q,  dv = P^T do
-// (delta is summed in fp32 from do and the stored output; in bf16 the output's rounding is in it, 2^-8 of |do| . |o| at most: forming it
-// from P and dP instead would take another pass over the states.)
+// (delta is summed in fp32 from do and the output.  In bf16 the forward of a training step forms the output from two planes of P and stores what
+// its rounding left as well: the rounded output alone makes dS that do not sum to zero, and dq and dk up to 1.9 times as far off as
+// their own rounding, 4.8 times with dS in one plane as well, where few states share the weight.  It costs 5 % of a training call, 427 -> 449
+// us at 4 x 1,280 x 2,560 x 128; dS in two planes for dq another 16 us.)
 // Two passes without atomics, so that the sums have one order: rows own dq (and write delta), states own dk and dv.  The
 // heads that share keys are rows of the same loop, so their gradients add up in the accumulator.
 
@@ -883,8 +946,8 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 // size -- dk and dv of 120 x 240 x 64 fp32: 4e-7 -> 1e-6 of the result.)
 constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
 
-// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  1,920 x 3,840 x 32 fp32 of 48 heads: 364 us = 187 TFLOP/s, matrix
-// units 0.55, vector units 0.51 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 119 us = 680 TFLOP/s, 0.26 and 0.21.
+// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  1,920 x 3,840 x 32 fp32 of 48 heads: 367 us = 185 TFLOP/s, matrix
+// units 0.55, vector units 0.50 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 144 us (119 with dS in one plane), 0.30 and 0.24.
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
@@ -926,6 +989,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
         qf[s] = load8(qrow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
         const Raw<NP> g = load8((const T *)a.go + dense, 16 * s + 8 * h, a.D, dwide, live);
         delta = dot8(g, load8((const T *)a.o + dense, 16 * s + 8 * h, a.D, dwide, live), delta);
+        if (NP == 1 && a.low) delta = dot8(g, load8((const T *)a.low + dense, 16 * s + 8 * h, a.D, dwide, live), delta);
         gf[s] = g.frag();
     }
     delta = other_half_sum(delta);
@@ -973,7 +1037,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, -lse)) * (start_at_delta(NP, DP) ? dp[i] : dp[i] - delta);
-            accumulate<NP>(dq, tk, 32 * t, s, lane);
+            accumulate<NP, NP == 1, false>(dq, tk, 32 * t, s, lane);
         }
         if (kTwo) {
             buf ^= 1;
@@ -991,9 +1055,9 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
 // are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS.  1,920 x 3,840 x 32 fp32 of 48 heads:
-// 504 us = 180 TFLOP/s, matrix units 0.53, vector units 0.54 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 218 us = 490 TFLOP/s, 0.19 and
+// 511 us = 177 TFLOP/s, matrix units 0.53, vector units 0.54 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 221 us = 490 TFLOP/s, 0.19 and
 // 0.17: dk, dv, k and v in registers leave one wave per SIMD.
-template <int NP, int DP, int BQ, bool WIDE>
+template <int NP, int DP, int BQ, bool WIDE, bool TWO>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
 {
     typedef typename Elem<NP>::T T;
@@ -1085,8 +1149,8 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
                 s[i] = __builtin_amdgcn_exp2f(exponent<NP>(s[i], a.c, row4(sl, i / 4)[i % 4]));
                 dp[i] = s[i] * (kStart ? dp[i] : dp[i] + row4(sd, i / 4)[i % 4]);
             }
-            accumulate<NP>(dv, tg, 32 * u, s, lane);
-            accumulate<NP>(dk, tq, 32 * u, dp, lane);
+            accumulate<NP, TWO, true>(dv, tg, 32 * u, s, lane);
+            accumulate<NP, TWO, false>(dk, tq, 32 * u, dp, lane);
         }
         if (kTwo) {
             buf ^= 1;
@@ -1178,6 +1242,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
     T *dst = MODE == 2 ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D
                        : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
     store4(dst, d, a.D, (a.D & 3) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (MODE == 0 && a.low) store_rest((T *)a.low + dense_row(b, r, hk, a), d, a.D, o, inv);
     if (MODE == 0 && a.lse && c == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -1239,6 +1304,7 @@ __global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per
     T *dst = MODE == 2 ? (T *)(which ? a.dv : a.dk) + (((int64_t)b * a.Lk + r) * a.Hk + hk) * a.D
                        : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
     store4(dst, d, a.D, quad, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (MODE == 0 && a.low) store_rest((T *)a.low + dense_row(b, r, hk, a), d, a.D, o, inv);
     if (MODE == 0 && a.lse && d == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
 }
 
@@ -1281,11 +1347,21 @@ bool wide_rows(const mvf_attn_desc &d)
     return (63 / G + 2) * q[1] + G * q[2] <= most && ((63 / G + 2) * d.Hq + G) * d.D <= most;
 }
 
+// Two planes of P and dS where one would be as much again as the result's own rounding, or more, and where they cost nothing:
+//   * the forward of a training step, whose output and its rest make delta;
+//   * dq: the dS of a row sum to zero and the keys that share its weight are alike, so that its terms cancel and their roundings do not
+//     (in one plane 1.5 times its own rounding, 2 in all, with normal queries and keys of 6 channels or four times larger queries of 16);
+//   * all of them below kSmall operations of the two forward products: an eager call of that size is the host's; in a captured training
+//     step they cost 1 - 4 us of 25 - 37 (60 x 120 and 120 x 240 x 64, 96 heads), 9 of 142 at one query and 15,360 states.
+// Everywhere they would cost 12 - 27 % (training 12 x 1,920 x 3,840 of 4 x 32: 335 -> 424 us; 4 x 1,280 x 2,560 of 8 x 128: 447 -> 499).
+constexpr double kSmall = 1e9;
+
 struct Plan {
     bool wide;                               // 16-byte loads
     int NP, DP, BK, BQ;
     int rtiles, ktiles;                      // workgroups along the rows, along the states
     int few;                                 // forward of at most 32 rows, the waves divide the states: 16 or 32 rows of a product; 0: more
+    bool two_f, two_k;                       // bf16: P and dS as two planes in the forward, dk / dv
     int fs, fper, qs, qper, ks, kper;        // parts of the reduction and tiles of a part: forward, dq (over the states), dkv (over the rows)
 };
 Plan plan_of(const mvf_attn_desc &d)
@@ -1298,6 +1374,9 @@ Plan plan_of(const mvf_attn_desc &d)
     p.BQ = tile_rows(p.NP, p.DP);
     const int R = d.Lq * (d.Hq / d.Hk);
     const int64_t bh = (int64_t)d.B * d.Hk;
+    const bool small = 4.0 * bh * R * d.Lk * d.D < kSmall;
+    p.two_f = p.NP == 1 && (d.out_low || small);
+    p.two_k = p.NP == 1 && small;
     p.rtiles = (R + 127) / 128;
     p.ktiles = (d.Lk + 127) / 128;
     p.few = R <= 16 ? 16 : R <= 32 ? 32 : 0;
@@ -1326,6 +1405,7 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
 {
     AttnArgs a = {};
     a.q = d.q; a.k = d.k; a.v = d.v;
+    a.low = d.dtype == MVF_DTYPE_BF16 ? d.out_low : nullptr;
     a.mask = d.key_mask; a.lens = d.kv_lens;
     for (int i = 0; i < 3; ++i) { a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i]; }
     a.wide = p.wide;
@@ -1338,25 +1418,36 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
     return a;
 }
 
+// a kernel by its last two arguments, 16-byte loads and two planes (of one-plane inputs alone)
+#define MVF_ATTN_LAUNCH(two, g, b, st, a, ...)                                                         \
+    do {                                                                                               \
+        if constexpr (NP == 1) {                                                                       \
+            if (two) {                                                                                 \
+                if ((a).wide) hipLaunchKernelGGL((__VA_ARGS__, true, true>), g, b, 0, st, a);          \
+                else hipLaunchKernelGGL((__VA_ARGS__, false, true>), g, b, 0, st, a);                  \
+                break;                                                                                 \
+            }                                                                                          \
+        }                                                                                              \
+        if ((a).wide) hipLaunchKernelGGL((__VA_ARGS__, true, false>), g, b, 0, st, a);                 \
+        else hipLaunchKernelGGL((__VA_ARGS__, false, false>), g, b, 0, st, a);                         \
+    } while (0)
 template <int NP, int DP>
-void launch_fwd(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_fwd(const AttnArgs &a, bool two, int64_t blocks, hipStream_t st)
 {
-    constexpr int BT = tile_states(NP, DP);
-    if (a.wide) hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_fwd<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    const dim3 g((unsigned)blocks), b(NT);
+    MVF_ATTN_LAUNCH(two, g, b, st, a, k_attn_fwd<NP, DP, tile_states(NP, DP));
 }
 template <int NP, int DP, int ROWS>
-void launch_few_rows(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_few_rows(const AttnArgs &a, bool two, int64_t blocks, hipStream_t st)
 {
     const dim3 g((unsigned)blocks), b(64 * few_waves_of(NP, DP, ROWS));
-    if (a.wide) hipLaunchKernelGGL((k_attn_few<NP, DP, ROWS, true>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((k_attn_few<NP, DP, ROWS, false>), g, b, 0, st, a);
+    MVF_ATTN_LAUNCH(two, g, b, st, a, k_attn_few<NP, DP, ROWS);
 }
 template <int NP, int DP>
-void launch_few(const AttnArgs &a, int rows, int64_t blocks, hipStream_t st)
+void launch_few(const AttnArgs &a, bool two, int rows, int64_t blocks, hipStream_t st)
 {
-    if (rows == 16) launch_few_rows<NP, DP, 16>(a, blocks, st);
-    else launch_few_rows<NP, DP, 32>(a, blocks, st);
+    if (rows == 16) launch_few_rows<NP, DP, 16>(a, two, blocks, st);
+    else launch_few_rows<NP, DP, 32>(a, two, blocks, st);
 }
 template <int NP, int DP>
 void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
@@ -1366,11 +1457,10 @@ void launch_dq(const AttnArgs &a, int64_t blocks, hipStream_t st)
     else hipLaunchKernelGGL((k_attn_dq<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
 }
 template <int NP, int DP>
-void launch_dkv(const AttnArgs &a, int64_t blocks, hipStream_t st)
+void launch_dkv(const AttnArgs &a, bool two, int64_t blocks, hipStream_t st)
 {
-    constexpr int BT = tile_rows(NP, DP);
-    if (a.wide) hipLaunchKernelGGL((k_attn_dkv<NP, DP, BT, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_dkv<NP, DP, BT, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    const dim3 g((unsigned)blocks), b(NT);
+    MVF_ATTN_LAUNCH(two, g, b, st, a, k_attn_dkv<NP, DP, tile_rows(NP, DP));
 }
 template <int MODE>
 void launch_join(const AttnArgs &a, int NP, int64_t rows, hipStream_t st)
@@ -1422,7 +1512,7 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     if (bad_desc(d)) return (int)hipErrorInvalidValue;
     if (d->B == 0 || d->Lq == 0) return 0;
     const Plan p = plan_of(*d);
-    if (!d->q || !out || (d->Lk > 0 && (!d->k || !d->v)) || (p.fs > 1 && !workspace) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 15))
+    if (!d->q || !out || (d->Lk > 0 && (!d->k || !d->v)) || (p.fs > 1 && !workspace) || (((uintptr_t)out | (uintptr_t)d->out_low | (uintptr_t)workspace) & 15))
         return (int)hipErrorInvalidValue;
     AttnArgs a = args_of(*d, p);
     const int64_t rows = (int64_t)d->B * d->Hq * d->Lq;
@@ -1433,8 +1523,8 @@ int mvf_cross_attention_fwd(const mvf_attn_desc *d, void *out, float *lse, void 
     a.part2 = p.fs > 1 ? a.part + p.fs * rows * d->D : nullptr;
     hipStream_t st = (hipStream_t)stream;
     ProfScope ps(MVF_PROF_ATTN_FWD, st, tensor_bytes(*d, 2 * rows + 2LL * d->B * d->Hk * d->Lk));
-    if (p.few) MVF_ATTN_PICK(launch_few, p, a, p.few, (int64_t)d->B * d->Hk * p.fs, st);
-    else MVF_ATTN_PICK(launch_fwd, p, a, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
+    if (p.few) MVF_ATTN_PICK(launch_few, p, a, p.two_f, p.few, (int64_t)d->B * d->Hk * p.fs, st);
+    else MVF_ATTN_PICK(launch_fwd, p, a, p.two_f, (int64_t)d->B * d->Hk * p.rtiles * p.fs, st);
     if (p.fs > 1) launch_join<0>(a, p.NP, rows, st);
     return hip_check_launch();
 }
@@ -1456,7 +1546,7 @@ int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float
     if (d->B == 0) return 0;
     if (d->Lq > 0 && (!d->q || !out || !lse || !g_out || !g_q || !workspace)) return (int)hipErrorInvalidValue;
     if (d->Lk > 0 && (!d->k || !d->v || !g_k != !g_v)) return (int)hipErrorInvalidValue;
-    if (((uintptr_t)out | (uintptr_t)g_out | (uintptr_t)g_q | (uintptr_t)g_k | (uintptr_t)g_v | (uintptr_t)workspace) & 15)
+    if (((uintptr_t)out | (uintptr_t)d->out_low | (uintptr_t)g_out | (uintptr_t)g_q | (uintptr_t)g_k | (uintptr_t)g_v | (uintptr_t)workspace) & 15)
         return (int)hipErrorInvalidValue;
     const Plan p = plan_of(*d);
     AttnArgs a = args_of(*d, p);
@@ -1474,7 +1564,7 @@ int mvf_cross_attention_bwd(const mvf_attn_desc *d, const void *out, const float
     }
     if (d->Lk > 0 && g_k) {
         a.tiles = p.ktiles; a.splits = p.ks; a.per = p.kper;
-        MVF_ATTN_PICK(launch_dkv, p, a, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
+        MVF_ATTN_PICK(launch_dkv, p, a, p.two_k, (int64_t)d->B * d->Hk * p.ktiles * p.ks, st);
         if (p.ks > 1) launch_join<2>(a, p.NP, 2 * states, st);
     }
     return hip_check_launch();

@@ -168,11 +168,16 @@ mvf_attn_desc attn_desc(const Tensor &q, const Tensor &k, const Tensor &v, const
     d.scale = (float)scale;
     return d;
 }
-Tensor attn_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &mask, const Tensor &lens, double scale, Tensor *lse)
+// lse, low: what a backward needs besides the output (low: of bfloat16), or null
+Tensor attn_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &mask, const Tensor &lens, double scale, Tensor *lse, Tensor *low)
 {
-    const mvf_attn_desc d = attn_desc(q, k, v, mask, lens, scale);
+    mvf_attn_desc d = attn_desc(q, k, v, mask, lens, scale);
     Tensor out = dense(q), ws;
     if (lse) *lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    if (low && d.dtype == MVF_DTYPE_BF16) {
+        *low = dense(q);
+        d.out_low = ptr(*low);
+    }
     if (const size_t n = api.attn_fwd_bytes(&d)) ws = at::empty({(int64_t)n}, q.options().dtype(at::kByte));
     check(api.attn_fwd(&d, ptr(out), lse ? (float *)ptr(*lse) : nullptr, ptr(ws), stream_now()), "cross_attention_fwd");
     return out;
@@ -183,9 +188,9 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
                           const std::optional<Tensor> &lens_, double scale)
     {
         const Tensor mask = or_none(mask_), lens = or_none(lens_);
-        Tensor lse;
-        const Tensor out = attn_forward(q, k, v, mask, lens, scale, &lse);
-        ctx->save_for_backward({q, k, v, mask, lens, out, lse});
+        Tensor lse, low;
+        const Tensor out = attn_forward(q, k, v, mask, lens, scale, &lse, &low);
+        ctx->save_for_backward({q, k, v, mask, lens, out, lse, low});
         ctx->saved_data["scale"] = scale;
         return out;
     }
@@ -194,8 +199,10 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
         once("cross_attention", grads);
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2];
-        const mvf_attn_desc d = attn_desc(q, k, v, s[3], s[4], ctx->saved_data["scale"].toDouble());
+        mvf_attn_desc d = attn_desc(q, k, v, s[3], s[4], ctx->saved_data["scale"].toDouble());
         const Tensor g = aligned(grads[0], q.scalar_type()), out = aligned(s[5], q.scalar_type()), lse = s[6].contiguous();
+        const Tensor low = s[7].defined() ? aligned(s[7], q.scalar_type()) : Tensor();
+        d.out_low = ptr(low);
         const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
         capturable("cross_attention", {{&q, need_q}, {&k, need_k}, {&v, need_v}});
         Tensor gq = dense(q), gk, gv;
@@ -234,7 +241,7 @@ Tensor cross_attention(Tensor q, Tensor k, Tensor v, std::optional<double> scale
     }
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
         return CrossAttention::apply(q, k, v, opt(mask), opt(lens), scale);
-    return attn_forward(q, k, v, mask, lens, scale, nullptr);
+    return attn_forward(q, k, v, mask, lens, scale, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------------------------------------- norm and rotation

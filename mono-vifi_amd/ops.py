@@ -1897,8 +1897,10 @@ def cross_attention(q, k, v, scale=None, key_mask=None, kv_lens=None):
     leaves it reaches lives on the default stream.  One query per sequence is the same call (the states are split over the chip).
     Refused under ``torch.jit.trace`` and other tracing, and for inputs with a forward gradient: the kernels are called past the
     dispatcher.  float32: products of values cut into three bfloat16 planes, 2^-21 of a product at most; infinities among the values
-    that count come out as infinities or NaN.  bfloat16: sums and the softmax are float32, its probabilities and the gradients of
-    the scores are rounded to bfloat16 where they enter a product, and the backward takes the output as rounded."""
+    that count come out as infinities or NaN.  bfloat16: sums and the softmax are float32; probabilities and the gradients of the
+    scores enter the products as 16 bits for the output of a call that will be differentiated and for dq, and in every call of at
+    most 1e9 operations; as bfloat16 for dk, dv and the output of larger calls under no_grad (whose last bits may so differ from
+    those of the same call in training)."""
     return nat.torch_ops().cross_attention(q, k, v, scale, key_mask, kv_lens)
 
 

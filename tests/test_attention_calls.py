@@ -254,7 +254,7 @@ def test_the_c_library_is_built_without_python(target):
     assert "/nonexistent" in make("torch").stdout                   # (the target that does need it)
 
 
-@pytest.mark.parametrize("what,change", [("ABI 15", lambda mp, nat: mp.setattr(nat, "ABI_VERSION", 99)),
+@pytest.mark.parametrize("what,change", [("ABI 16", lambda mp, nat: mp.setattr(nat, "ABI_VERSION", 99)),
                                          ("torch 2", lambda mp, nat: mp.setattr(torch, "__version__", "1.0.0+other"))])
 def test_an_extension_of_another_build_is_not_loaded(monkeypatch, what, change):
     from mono_vifi_amd import _native as nat
@@ -294,6 +294,15 @@ def test_attention_sizes_at_the_limit_of_a_launch(kw, most):
         assert lib.mvf_cross_attention_bwd_workspace_bytes(C.byref(beyond)) == 0
         assert lib.mvf_cross_attention_fwd(C.byref(beyond), P, None, P, None) == 1
         assert lib.mvf_cross_attention_bwd(C.byref(beyond), P, P, P, P, P, P, P, None) == 1
+
+
+def test_the_rest_of_the_output_has_to_be_aligned():
+    import ctypes as C
+    from mono_vifi_amd import _native as nat
+    d, P, keep = c_call(nat.AttnDesc, dtype=1)
+    d.out_low = P + 4
+    assert nat.lib().mvf_cross_attention_fwd(C.byref(d), P, None, P, None) == 1
+    assert nat.lib().mvf_cross_attention_bwd(C.byref(d), P, P, P, P, P, P, P, None) == 1
 
 
 # a workgroup of 256 threads takes 256 rows of one pair of channels, 64 of 4 lanes, 4 of 64
@@ -458,3 +467,63 @@ def test_far_positions_are_off_by_their_frequencies_rounding_alone(bits, base):
     assert ((got - want).abs() <= size * ((D + 24) * 2.0 ** -24 + off) + 2.0 ** -24 * want.abs()).all()
     # and at far positions the bound itself says something: not more than a hundredth of a radian up to 2^48
     assert bits > 48 or float(off.max()) < 1e-2
+
+
+# ------------------------------------------------------------------------------------------------ bfloat16: how far beyond the result's own rounding
+# 1 is the error that rounding the exact result makes (relative 2-norm).  P and dS in two planes (2^-16 of a term) and delta from the output
+# and its rest add a hundredth of that; P or dS in one plane are terms rounded to as many bits as the result, independently: sqrt(2), and a few
+# percent where the terms cancel by chance.
+def beyond_rounding(got, want):
+    return [float((a.double() - b).norm() / (b.bfloat16().double() - b).norm()) for a, b in zip(got, want)]
+
+
+def bf16_call(B, Lq, Lk, Hq, Hk, D, spread=1.0):
+    q, k, v, go = (x.bfloat16() for x in normal(3, B, Lq, Lk, Hq, Hk, D, device="cuda"))
+    q = (q * spread).bfloat16()
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    got = [out.detach()] + list(torch.autograd.grad(out, leaves, go))
+    with torch.no_grad():
+        alone = ops.cross_attention(*leaves)
+    want = defined(q, k, v, go)
+    return beyond_rounding(got, want), beyond_rounding([alone], want[:1])[0]
+
+
+@gpu
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+@pytest.mark.parametrize("D", [6, 16, 28, 64, 80, 128])
+@pytest.mark.parametrize("form", [(4, 100, 8, 3, 3), (4, 100, 40, 4, 2), (10, 281, 72, 3, 3), (2, 600, 700, 2, 2), (2, 3, 2500, 4, 1), (3, 20, 600, 1, 1), (8, 4, 30, 8, 2)], ids=str)
+def test_bf16_gradients_of_few_states_and_narrow_heads(form, D, spread):
+    """Small calls: no precision is lost beyond the rounding of the results, also where a query attends to few states."""
+    got, alone = bf16_call(*form, D, spread=spread)
+    assert max(got) <= 1.05 and alone <= 1.05, (got, alone)
+
+
+@gpu
+@pytest.mark.parametrize("D,Lq,Lk", [(6, 3000, 4000), (12, 2000, 4000), (16, 4000, 2000), (32, 2000, 2100), (64, 1300, 1100), (96, 1200, 1000), (128, 1000, 1300)])
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+def test_bf16_gradients_of_larger_calls(D, Lq, Lk, spread):
+    """The output of a training step and dq in two planes, the others in one."""
+    got, alone = bf16_call(2, Lq, Lk, 2, 2, D, spread=spread)
+    assert 4 * 4 * Lq * Lk * D > 1e9                                  # (where one plane begins)
+    bars = [1.05, 1.05, 1.5, 1.5]
+    assert all(a <= b for a, b in zip(got, bars)) and alone <= 1.5, (got, alone)
+
+
+@gpu
+@pytest.mark.parametrize("form", [(2, 40, 70, 2, 2, 32), (1, 3, 300, 4, 2, 64), (1, 20, 300, 1, 1, 80), (1, 2, 5000, 2, 1, 64), (2, 600, 700, 2, 2, 28)], ids=str)
+def test_bf16_infinities_that_count_come_out_as_infinities(form):
+    """Every probability is positive: an infinite value of a state is infinite in that channel of every query that reads it, and nothing else
+    changes."""
+    q, k, v, _ = (x.bfloat16() for x in normal(4, *form, device="cuda"))
+    D, group = form[-1], form[3] // form[4]
+    for grad in (False, True):
+        clean = ops.cross_attention(q.detach().requires_grad_(grad), k, v)
+        for value in (float("inf"), float("-inf")):
+            w = v.clone()
+            w[0, form[2] // 2, 0, D - 3] = value
+            out = ops.cross_attention(q.detach().requires_grad_(grad), k, w)
+            assert (out[0, :, :group, D - 3] == value).all()
+            rest = torch.ones_like(out, dtype=torch.bool)
+            rest[0, :, :group, D - 3] = False
+            assert torch.equal(out[rest], clean[rest])
