@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MVF_ABI_VERSION 16
+#define MVF_ABI_VERSION 17
 
 #if defined(__GNUC__)
 #define MVF_API __attribute__((visibility("default")))
@@ -596,6 +596,8 @@ typedef struct mvf_attn_desc {
     float scale;                    /* > 0 */
     void *out_low;                  /* nullable [B,Lq,Hq,D] bf16, contiguous, 16-byte aligned: what the rounding of out to bf16 left.  The forward
                                      * of a training step writes it (and then keeps P to 16 bits), its backward reads it; not used in fp32 */
+    float *inv_sum;                 /* nullable, B*Hq*Lq floats as lse: 1 / the sum of a row's exponentials, of which lse is then the reference
+                                     * alone.  The forward of a training step writes it, its backward reads it (both or neither); not used in bf16 */
 } mvf_attn_desc;
 /* out [B,Lq,Hq,D] contiguous = softmax(scale q k^T over the states that count) v; zeros where none counts.
  * States that do not count are never multiplied (their memory may hold anything).  lse (nullable, for the

@@ -12,7 +12,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MVF_HOTPATH_LIB: developer knob (kernel variant builds); the product loads the in-tree library
 LIB_PATH = os.environ.get("MVF_HOTPATH_LIB") or os.path.join(_HERE, "lib", "libmvf_hotpath.so")
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 NO_SSIM, AVG_REPROJ, NO_AUTOMASK = 1, 2, 4
 MAX_SRC = 4
@@ -77,7 +77,7 @@ class AttnDesc(C.Structure):
     _fields_ = [
         ("q", _vp), ("k", _vp), ("v", _vp), ("key_mask", _vp), ("kv_lens", _vp),
         ("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("v_stride", _i64 * 3), ("mask_stride", _i64 * 2),
-        ("B", _i), ("Lq", _i), ("Lk", _i), ("Hq", _i), ("Hk", _i), ("D", _i), ("dtype", _i), ("scale", _f), ("out_low", _vp),
+        ("B", _i), ("Lq", _i), ("Lk", _i), ("Hq", _i), ("Hk", _i), ("D", _i), ("dtype", _i), ("scale", _f), ("out_low", _vp), ("inv_sum", _vp),
     ]
 
 

@@ -39,7 +39,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NT = 256;            // four waves
 constexpr int PADE = 8;            // bf16 elements appended to an LDS row: rows 16 bytes apart modulo 128
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Staged tiles: two buffers (one barrier per tile) for one plane, one buffer (two barriers) for three, whose tiles would halve
 // the number of resident workgroups (1,920 x 3,840 x 32 fp32 forward: 264 against 285 us)
@@ -122,6 +122,20 @@ MVF_DEV f32x16 mma(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
 }
 
+// The same bits as mma(b, a) with rows and columns exchanged: the terms in the other order.
+template <int NP>
+MVF_DEV f32x16 mma_exchanged(const Frag<NP> &a, const Frag<NP> &b, f32x16 c)
+{
+    if constexpr (NP == 3) {
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], c, 0, 0, 0);
+    }
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+
 // the same for 16 x 16 tiles: 32 channels or states per product
 template <int NP>
 MVF_DEV f32x4 mma(const Frag<NP> &a, const Frag<NP> &b, f32x4 c)
@@ -169,8 +183,10 @@ struct Raw<3> {
         return split8<3>(x);
     }
 };
-// The factor c of the exponent: three planes take it into q (or k) before it is cut, one rounding of fp32 among those of the
-// products, so that the scores come out of the matrix units ready; one plane would round the product to bf16.
+// The factor c of the exponent: three planes take it into q before it is cut, one rounding of fp32 among those of the products, so
+// that the scores come out of the matrix units ready; one plane would round the product to bf16.  In three planes all kernels
+// of a training step form the same bits of a score, by the same products in the same order: a score of 150 rounds by 8e-6, and a
+// probability whose exponent and reference rounded apart would be off by that (dv at scores of 150: 1.2e-5 of the result).
 template <int NP>
 MVF_DEV float exponent(float s, float c, float minus) { return NP == 3 ? s + minus : fmaf(s, c, minus); }
 // channels d0 .. d0 + 7 of a row of D channels (zeros behind D, or if the row is not `live`); `wide`: rows are 16-byte aligned
@@ -291,7 +307,7 @@ struct Tile {
 struct AttnArgs {
     const void *q, *k, *v, *o, *go;
     void *out, *low, *dq, *dk, *dv;           // low: what the rounding of out left (bf16 training), or null
-    float *lse, *delta, *part, *part2;
+    float *lse, *inv, *delta, *part, *part2;  // inv: 1 / the softmax sum (fp32), or null: in lse
     const uint8_t *mask;
     const int32_t *lens;
     int64_t qs[3], ks[3], vs[3], ms[2];       // batch, token, head strides in elements; mask: batch, state
@@ -383,6 +399,14 @@ struct Flight {
         for (int i = 0; i < N; ++i)
             if (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) t.put(row_of(i), chan_of(i) / 8, r[i].frag());
     }
+    // the same, rows times f(i) (three planes)
+    template <typename F>
+    MVF_DEV void commit(Tile<NP, ROWS, DP> &t, F f) const
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (CHUNKS % NT == 0 || i * NT + threadIdx.x < CHUNKS) t.put(row_of(i), chan_of(i) / 8, r[i].frag_scaled(f(i)));
+    }
 };
 template <bool WIDE>
 struct Stride;                    // a stride, as wide as the offsets within a tile have to be
@@ -415,6 +439,17 @@ MVF_DEV void stream(L load, M mul)
         mul(i, f[i]);
         MVF_PIN();
     }
+}
+
+// What the backward needs of a row's softmax.  lse: the reference of its exponentials, and 1 / their sum beside it (fp32) -- or both in one
+// number, the log2 of the sum: in fp32 that rounds at the size of the scores, the same way for all of the row (2^-17 of P at scores of
+// 150), where m is a score and s - m is exact where it matters.  INFINITY: no state counts, every exponential is zero.
+template <bool F32>
+MVF_DEV void store_softmax(const AttnArgs &a, int64_t at, float m, float l)
+{
+    const bool apart = F32 && a.inv;
+    a.lse[at] = l == 0.0f ? INFINITY : apart ? m : m + __builtin_amdgcn_logf(l);
+    if (apart) a.inv[at] = l == 0.0f ? 1.0f : 1.0f / l;
 }
 
 // The tiles of states a workgroup walks: [j, end) in steps of BK, those without a state that counts left out.  The same in
@@ -722,14 +757,15 @@ __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     store_cols<DT>((T *)a.out + dense_row(b, r, hk, a), o, inv, a.D, (a.D & 3) == 0, h);
     if (TWO && a.low) store_cols_rest<DT>((T *)a.low + dense_row(b, r, hk, a), o, inv, a.D, h);
-    if (a.lse && h == 0) a.lse[(int64_t)bh * a.R + r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (a.lse && h == 0) store_softmax<NP == 3>(a, (int64_t)bh * a.R + r, m, l);
 }
 
 // The same for at most 32 rows (a few queries, or one with the heads of its group): four row tiles would leave three waves of a
 // workgroup idle, so here the waves share the rows and divide the states, 32 each in turn, every wave on its own: keys go from
 // memory straight to the registers that hold the left operand (32 bytes of a row per lane), values through a tile of the
 // wave's own, the next 32 states are in flight meanwhile, and no barrier until the partial results are joined in LDS.
-// ROWS: the rows of a product.  At most 16 rows take 16 x 16 x 32 products, half of the matrix work and of the registers of q and o.
+// ROWS: the rows of a product.  At most 16 rows take 16 x 16 x 32 products, half of the matrix work and of the registers of q and o -- but not
+// in the forward of an fp32 training step, whose backward has to form the same bits of the scores.
 // Bound by the bytes of keys and values: 3.8 TB/s at 15,360 bf16 states (4 x 2 heads of 64: 8.2 us), 3.9 at 40,001 fp32 states (2 x
 // 3 heads of 80: 35 us; 43 with 32-row products, 92 by row tiles).
 // Eight waves where the registers of 16-row products let two waves into a SIMD and the loads are fp32 (5 x 40,001 x 80: 41.6 us, 43.0
@@ -926,13 +962,13 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
             a.part2[2 * y] = top;
             a.part2[2 * y + 1] = sum;
         } else if (a.lse) {
-            a.lse[(int64_t)bh * a.R + r] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+            store_softmax<NP == 3>(a, (int64_t)bh * a.R + r, top, sum);
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------- backward
-// P is recomputed from the stored log2 of the softmax sum; delta = do . o is what the softmax subtracts from dP:
+// P is recomputed from the reference and the sum of the row's exponentials (store_softmax); delta = do . o is what the softmax subtracts from dP:
 //     dS = P (dP - delta),  dP = do V^T,  dq = scale dS K,  dk = scale dS^T q,  dv = P^T do
 // (delta is summed in fp32 from do and the output.  In bf16 the forward of a training step forms the output from two planes of P and stores what
 // its rounding left as well: the rounded output alone makes dS that do not sum to zero, and dq and dk up to 1.9 times as far off as
@@ -994,6 +1030,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     }
     delta = other_half_sum(delta);
     const float lse = live ? a.lse[(int64_t)bh * a.R + r] : INFINITY;
+    const float out = NP == 3 && a.inv && live ? a.scale * a.inv[(int64_t)bh * a.R + r] : a.scale;      // of the sums below, the row's dq
     if (live && part == 0 && h == 0) a.delta[(int64_t)bh * a.R + r] = delta;
     f32x16 dq[DT], minus_delta;
 #pragma unroll
@@ -1047,10 +1084,10 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
     if (!live) return;
     if (a.splits > 1) {
         const int64_t y = ((int64_t)part * a.B * a.Hk + bh) * a.R + r;
-        store_cols<DT>(a.part + y * a.D, dq, a.scale, a.D, (a.D & 3) == 0, h);
+        store_cols<DT>(a.part + y * a.D, dq, out, a.D, (a.D & 3) == 0, h);
         return;
     }
-    store_cols<DT>((T *)a.dq + dense, dq, a.scale, a.D, (a.D & 3) == 0, h);
+    store_cols<DT>((T *)a.dq + dense, dq, out, a.D, (a.D & 3) == 0, h);
 }
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
@@ -1074,7 +1111,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     const int r1 = tile * 128 < n ? (int)min((int64_t)a.R, (int64_t)(part + 1) * a.per * BQ) : 0;
     int r0 = part * a.per * BQ;
     Flight<NP, BQ, DP, WIDE> fq, fg;
-    float pl = 0.0f, pd = 0.0f;
+    float pl = 0.0f, pd = 0.0f, pf[fg.N];                        // pf: what do and delta of a row are multiplied with, in place of P
     typedef typename Stride<WIDE>::T Off;
     const Off qs1 = a.qs[1], qs2 = a.qs[2], gs1 = (int64_t)a.Hq * a.D, gs2 = a.D;
     const float invG = 1.0f / (float)a.G;
@@ -1093,13 +1130,26 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
             const int r = r0 + threadIdx.x;
             pl = r < a.R ? -a.lse[(int64_t)bh * a.R + r] : -INFINITY;          // rows behind the last: P = 0
             pd = r < a.R ? -a.delta[(int64_t)bh * a.R + r] : 0.0f;
+            if (NP == 3 && a.inv && r < a.R) pd *= a.inv[(int64_t)bh * a.R + r];
+        }
+        if constexpr (NP == 3) {
+#pragma unroll
+            for (int i = 0; i < fg.N; ++i) {
+                const int r = r0 + fg.row_of(i);
+                pf[i] = a.inv && r < a.R ? a.inv[(int64_t)bh * a.R + r] : 1.0f;
+            }
         }
     };
     constexpr bool kTwo = buffers(NP) == 2;
     int buf = 0;
     auto commit = [&] {
-        fq.commit(tile_q[buf]);
-        fg.commit(tile_g[buf]);
+        if constexpr (NP == 3) {
+            fq.commit(tile_q[buf], [&](int) { return a.c; });
+            fg.commit(tile_g[buf], [&](int i) { return pf[i]; });
+        } else {
+            fq.commit(tile_q[buf]);
+            fg.commit(tile_g[buf]);
+        }
         if (threadIdx.x < BQ) {
             row_lse[buf][threadIdx.x] = pl;
             row_delta[buf][threadIdx.x] = pd;
@@ -1112,7 +1162,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     Frag<NP> kf[KS], vf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        kf[s] = load8(krow, 16 * s + 8 * h, a.D, WIDE, live).frag_scaled(a.c);
+        kf[s] = load_frag<NP>(krow, 16 * s + 8 * h, a.D, WIDE, live);
         vf[s] = load_frag<NP>(vrow, 16 * s + 8 * h, a.D, WIDE, live);
     }
     f32x16 dk[DT], dv[DT];
@@ -1141,7 +1191,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
             stream<NP, 2 * KS>([&](int i) { return (i % 2 ? tg : tq).rows(32 * u, 16 * (i / 2), lane); },
                                [&](int i, const Frag<NP> &f) {
                                    if (i % 2) dp = mma(f, vf[i / 2], dp);
-                                   else s = mma(f, kf[i / 2], s);
+                                   else s = mma_exchanged(f, kf[i / 2], s);
                                });
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -1158,6 +1208,7 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
         }
     }
     if (j >= a.Lk) return;
+    const float of_dk = NP == 3 ? kLn2 : a.scale;                 // (three planes: the rows carry scale * log2(e))
     if (!live) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) dk[d] = dv[d] = f32x16{};
@@ -1165,12 +1216,12 @@ __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
     if (a.splits > 1) {
         const int64_t n1 = (int64_t)a.B * a.Hk * a.Lk * a.D, y = ((int64_t)bh * a.Lk + j) * a.D + 2 * part * n1;
         const bool pw = (a.D & 3) == 0;
-        store_cols<DT>(a.part + y, dk, a.scale, a.D, pw, h);
+        store_cols<DT>(a.part + y, dk, of_dk, a.D, pw, h);
         store_cols<DT>(a.part + y + n1, dv, 1.0f, a.D, pw, h);
         return;
     }
     const int64_t y = (((int64_t)b * a.Lk + j) * a.Hk + hk) * a.D;
-    store_cols<DT>((T *)a.dk + y, dk, a.scale, a.D, (a.D & 3) == 0, h);
+    store_cols<DT>((T *)a.dk + y, dk, of_dk, a.D, (a.D & 3) == 0, h);
     store_cols<DT>((T *)a.dv + y, dv, 1.0f, a.D, (a.D & 3) == 0, h);
 }
 
@@ -1243,7 +1294,7 @@ __global__ void __launch_bounds__(NT) k_attn_join(const AttnArgs a, int per, int
                        : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
     store4(dst, d, a.D, (a.D & 3) == 0, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     if (MODE == 0 && a.low) store_rest((T *)a.low + dense_row(b, r, hk, a), d, a.D, o, inv);
-    if (MODE == 0 && a.lse && c == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (MODE == 0 && a.lse && c == 0) store_softmax<sizeof(T) == 4>(a, w, m, l);
 }
 
 // The same for few parts (at most kFlat): a lane adds all parts of its four channels, without a word to the others.  (Two parts of
@@ -1305,7 +1356,7 @@ __global__ void __launch_bounds__(NT) k_attn_join_flat(const AttnArgs a, int per
                        : (T *)(MODE == 0 ? a.out : a.dq) + dense_row(b, r, hk, a);
     store4(dst, d, a.D, quad, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     if (MODE == 0 && a.low) store_rest((T *)a.low + dense_row(b, r, hk, a), d, a.D, o, inv);
-    if (MODE == 0 && a.lse && d == 0) a.lse[w] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (MODE == 0 && a.lse && d == 0) store_softmax<sizeof(T) == 4>(a, w, m, l);
 }
 
 // ------------------------------------------------------------------------------------------------- host side
@@ -1379,7 +1430,7 @@ Plan plan_of(const mvf_attn_desc &d)
     p.two_k = p.NP == 1 && small;
     p.rtiles = (R + 127) / 128;
     p.ktiles = (d.Lk + 127) / 128;
-    p.few = R <= 16 ? 16 : R <= 32 ? 32 : 0;
+    p.few = R <= 16 && !(p.NP == 3 && d.inv_sum) ? 16 : R <= 32 ? 32 : 0;       // (an fp32 backward forms the scores of 32-row products)
     split_of(bh * p.rtiles, (d.Lk + p.BK - 1) / p.BK, 4, p.qs, p.qper);
     const int turn = 32 * few_waves_of(p.NP, p.DP, p.few);
     if (p.few) split_of(bh, (d.Lk + turn - 1) / turn, 256 / turn, p.fs, p.fper);
@@ -1406,6 +1457,7 @@ AttnArgs args_of(const mvf_attn_desc &d, const Plan &p)
     AttnArgs a = {};
     a.q = d.q; a.k = d.k; a.v = d.v;
     a.low = d.dtype == MVF_DTYPE_BF16 ? d.out_low : nullptr;
+    a.inv = d.dtype == MVF_DTYPE_F32 ? d.inv_sum : nullptr;
     a.mask = d.key_mask; a.lens = d.kv_lens;
     for (int i = 0; i < 3; ++i) { a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i]; }
     a.wide = p.wide;

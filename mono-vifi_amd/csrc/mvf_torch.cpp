@@ -168,12 +168,13 @@ mvf_attn_desc attn_desc(const Tensor &q, const Tensor &k, const Tensor &v, const
     d.scale = (float)scale;
     return d;
 }
-// lse, low: what a backward needs besides the output (low: of bfloat16), or null
+// lse, low: what a backward needs besides the output, or null (low: the rest of a bfloat16 output; lse of float32: and 1 / the sums behind it)
 Tensor attn_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &mask, const Tensor &lens, double scale, Tensor *lse, Tensor *low)
 {
     mvf_attn_desc d = attn_desc(q, k, v, mask, lens, scale);
     Tensor out = dense(q), ws;
-    if (lse) *lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    if (lse) *lse = at::empty({d.dtype == MVF_DTYPE_F32 ? 2 : 1, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+    if (lse && d.dtype == MVF_DTYPE_F32) d.inv_sum = (float *)ptr(*lse) + lse->numel() / 2;
     if (low && d.dtype == MVF_DTYPE_BF16) {
         *low = dense(q);
         d.out_low = ptr(*low);
@@ -203,6 +204,7 @@ struct CrossAttention : torch::autograd::Function<CrossAttention> {
         const Tensor g = aligned(grads[0], q.scalar_type()), out = aligned(s[5], q.scalar_type()), lse = s[6].contiguous();
         const Tensor low = s[7].defined() ? aligned(s[7], q.scalar_type()) : Tensor();
         d.out_low = ptr(low);
+        if (d.dtype == MVF_DTYPE_F32) d.inv_sum = (float *)ptr(lse) + lse.numel() / 2;
         const bool need_q = ctx->needs_input_grad(0), need_k = ctx->needs_input_grad(1), need_v = ctx->needs_input_grad(2);
         capturable("cross_attention", {{&q, need_q}, {&k, need_k}, {&v, need_v}});
         Tensor gq = dense(q), gk, gv;

@@ -254,7 +254,7 @@ def test_the_c_library_is_built_without_python(target):
     assert "/nonexistent" in make("torch").stdout                   # (the target that does need it)
 
 
-@pytest.mark.parametrize("what,change", [("ABI 16", lambda mp, nat: mp.setattr(nat, "ABI_VERSION", 99)),
+@pytest.mark.parametrize("what,change", [("ABI 17", lambda mp, nat: mp.setattr(nat, "ABI_VERSION", 99)),
                                          ("torch 2", lambda mp, nat: mp.setattr(torch, "__version__", "1.0.0+other"))])
 def test_an_extension_of_another_build_is_not_loaded(monkeypatch, what, change):
     from mono_vifi_amd import _native as nat
@@ -527,3 +527,63 @@ def test_bf16_infinities_that_count_come_out_as_infinities(form):
             rest = torch.ones_like(out, dtype=torch.bool)
             rest[0, :, :group, D - 3] = False
             assert torch.equal(out[rest], clean[rest])
+
+
+# ------------------------------------------------------------------------------------------------ fp32: scores of a trained network's size
+def plain_fp32(q, k, v, go):
+    """[out, dq, dk, dv] from elementary operations in fp32, probabilities normalised before the products."""
+    xs = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    qh, kh, vh = by_heads(*xs)
+    s = qh @ kh.transpose(-1, -2).contiguous() * q.shape[-1] ** -0.5
+    e = torch.exp(s - s.detach().amax(-1, keepdim=True))
+    out = ((e / e.sum(-1, keepdim=True)) @ vh.contiguous()).permute(0, 2, 1, 3)
+    return [out.detach()] + list(torch.autograd.grad(out, xs, go))
+
+
+@gpu
+@pytest.mark.parametrize("spread", [1.0, 4.0, 10.0, 30.0])
+@pytest.mark.parametrize("form", [(2, 300, 400, 4, 2, 64), (2, 300, 40, 3, 3, 6), (2, 200, 3000, 2, 2, 32), (2, 5, 3000, 4, 2, 64), (1, 600, 700, 2, 2, 128),
+                                  (2, 20, 900, 1, 1, 96), (2, 90, 130, 2, 2, 57)], ids=str)
+def test_fp32_gradients_at_large_scores(form, spread):
+    """Scores up to 150: no further off than three times the plain form in fp32, or 1e-6.  Both round the scores, each in its order (2^-24 of
+    150, 8e-6 of a probability), and normalise what they got, so that the roundings of a row's largest scores cancel; three times for the
+    random choice of the rows that weigh most.  Kernels that rounded a score apart in the forward and the backward are up to 10 times off."""
+    q, k, v, go = normal(5, *form, device="cuda")
+    q = q * spread
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    want = defined(q, k, v, go)
+    got = deviations([out.detach()] + list(torch.autograd.grad(out, leaves, go)), want)
+    plain = deviations(plain_fp32(q, k, v, go), want)
+    assert all(a <= max(1e-6, 3 * b) for a, b in zip(got, plain)), (got, plain)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("form", [(2, 130, 200, 2, 1, 32), (1, 3, 900, 4, 2, 64), (2, 600, 700, 2, 2, 28)], ids=str)
+def test_the_c_entry_points_without_their_optional_tensors(form, dtype):
+    """lse alone, as one number per row: the same gradients but for its rounding (2^-24 of scores below 16) and, in bf16, that of the output in
+    delta; with the optional tensors, the bits of the torch function."""
+    import ctypes as C
+    from mono_vifi_amd import _native as nat
+    lib, (B, Lq, Lk, Hq, Hk, D) = nat.lib(), form
+    q, k, v, go = (x.to(dtype) for x in normal(6, *form, device="cuda"))
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def call(optional):
+        d = nat.AttnDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=q.stride()[:3], k_stride=k.stride()[:3], v_stride=v.stride()[:3],
+                         B=B, Lq=Lq, Lk=Lk, Hq=Hq, Hk=Hk, D=D, dtype=nat.DTYPE_F32 if dtype == torch.float32 else nat.DTYPE_BF16, scale=D ** -0.5)
+        rest, lse = torch.empty_like(q), torch.empty(2, B, Lq, Hq, device="cuda")
+        if optional:
+            d.out_low, d.inv_sum = rest.data_ptr(), lse[1].data_ptr()
+        out, gq, gk, gv = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        for size, entry, args in ((lib.mvf_cross_attention_fwd_workspace_bytes, lib.mvf_cross_attention_fwd, (out, lse)),
+                                  (lib.mvf_cross_attention_bwd_workspace_bytes, lib.mvf_cross_attention_bwd, (out, lse, go, gq, gk, gv))):
+            ws = torch.empty(size(C.byref(d)) + 16, dtype=torch.uint8, device="cuda")
+            assert entry(C.byref(d), *(x.data_ptr() for x in args), ws.data_ptr(), stream) == 0
+        return [out, gq, gk, gv]
+    want = defined(q, k, v, go)
+    leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+    o = ops.cross_attention(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(call(True), [o] + list(torch.autograd.grad(o, leaves, go))))
+    assert max(deviations(call(False), want)) <= (BAR if dtype == torch.float32 else 3 * 2.0 ** -8)
