@@ -263,6 +263,7 @@ def torch_ops():
     global _torch_ops
     if _torch_ops is None:
         import importlib.util
+        import re
         import torch
         handle = lib()
         path, make = os.path.join(_HERE, "lib", "_mvf_torch.so"), "`python __graft_entry__.py` (or `make -C mono-vifi_amd/csrc torch`)"
@@ -274,7 +275,7 @@ def torch_ops():
             spec.loader.exec_module(module)
         except ImportError as e:
             raise NativeLibraryError(f"{path} does not load with torch {torch.__version__}: run {make}") from e
-        built, want = [(getattr(module, "abi", None), getattr(module, "torch", None)), (ABI_VERSION, torch.__version__.split("+")[0])]
+        built, want = [(getattr(module, "abi", None), getattr(module, "torch", None)), (ABI_VERSION, ".".join(re.findall(r"\d+", torch.__version__)[:3]))]
         if built != want:
             raise NativeLibraryError(f"{path} was built for ABI {built[0]} and torch {built[1]}, this is ABI {want[0]} and torch {want[1]}: "
                                      f"run {make}")
