@@ -616,10 +616,10 @@ MVF_DEV void accumulate(f32x16 (&acc)[DT], const Tile<NP, ROWS, DP> &t, int r0, 
 // grid: (batch x key head) major, then the part of the states, then the row tile (4 waves x 32 rows).  Two tile buffers: the
 // loads of the next tile are issued at the top, written to the other buffer at the bottom, one barrier per tile (three planes:
 // one buffer).  (Times here and below are of kernel traces; among repeated calls the large ones are 3 - 10 % shorter.)
-// 1,920 x 3,840 x 32 fp32 of 48 heads: 281 - 285 us = 160 TFLOP/s (960 in bf16), the vector units active 0.61 of the time (exponentials,
-// cutting into planes) and the matrix units 0.47.  7,680 x 15,360 x 64 bf16 of 8 heads: 343 - 359 us = 690 TFLOP/s, vector 0.45, matrix 0.30: two
+// 1,920 x 3,840 x 32 fp32 of 48 heads: 281 - 288 us = 160 TFLOP/s (960 in bf16), the vector units active 0.60 of the time (exponentials,
+// cutting into planes) and the matrix units 0.46.  7,680 x 15,360 x 64 bf16 of 8 heads: 340 - 359 us = 690 TFLOP/s, vector 0.45, matrix 0.29: two
 // waves per SIMD wait, a third of their cycles for an instruction to be taken.  1,280 x 2,560 x 128 bf16 of 32 heads: 94 us = 570 TFLOP/s, in
-// training (P in two planes) 117; vector 0.24, matrix 0.27: 320 workgroups on 256 CUs, one wave per SIMD.
+// training (P in two planes) 116; vector 0.26, matrix 0.27: 320 workgroups on 256 CUs, one wave per SIMD.
 template <int NP, int DP, int BK, bool WIDE, bool TWO>
 __global__ void __launch_bounds__(NT) k_attn_fwd(const AttnArgs a)
 {
@@ -982,8 +982,8 @@ __global__ void __launch_bounds__(64 * few_waves_of(NP, DP, ROWS)) k_attn_few(co
 // size -- dk and dv of 120 x 240 x 64 fp32: 4e-7 -> 1e-6 of the result.)
 constexpr bool start_at_delta(int NP, int DP) { return NP == 3 || DP <= 64; }
 
-// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  1,920 x 3,840 x 32 fp32 of 48 heads: 367 us = 185 TFLOP/s, matrix
-// units 0.55, vector units 0.50 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 144 us (119 with dS in one plane), 0.30 and 0.24.
+// grid as the forward's: S^T and dP^T of a tile, then dq^T += K^T dS^T.  1,920 x 3,840 x 32 fp32 of 48 heads: 367 - 375 us = 183 TFLOP/s, matrix
+// units 0.55, vector units 0.50 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 143 us (119 with dS in one plane), 0.30 and 0.24.
 template <int NP, int DP, int BK, bool WIDE>
 __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 {
@@ -1092,7 +1092,7 @@ __global__ void __launch_bounds__(NT) k_attn_dq(const AttnArgs a)
 
 // grid: (batch x key head) major, then the part of the rows, then the state tile (4 waves x 32 states).  Row tiles of q and do
 // are staged; S and dP have this wave's states as columns, dv^T += do^T P, dk^T += q^T dS.  1,920 x 3,840 x 32 fp32 of 48 heads:
-// 511 us = 177 TFLOP/s, matrix units 0.53, vector units 0.54 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 221 us = 490 TFLOP/s, 0.19 and
+// 522 us = 174 TFLOP/s, matrix units 0.51, vector units 0.53 of the time; 1,280 x 2,560 x 128 bf16 of 32 heads: 217 us = 490 TFLOP/s, 0.19 and
 // 0.17: dk, dv, k and v in registers leave one wave per SIMD.
 template <int NP, int DP, int BQ, bool WIDE, bool TWO>
 __global__ void __launch_bounds__(NT) k_attn_dkv(const AttnArgs a)
